@@ -80,6 +80,10 @@ LIB_SOURCES = [
     "csrc/gemm/kernels_deepk.hip",
     "csrc/api/c_api.cpp",
     "csrc/api/scratch.hip",
+    "csrc/api/train_api.cpp",
+    "csrc/train/clip.hip",
+    "csrc/train/cross_entropy.hip",
+    "csrc/train/route.hip",
 ]
 TESTING_SOURCES = ["csrc/api/testing_api.cpp"]
 
@@ -169,12 +173,14 @@ def torch_flags() -> tuple[list[str], list[str]]:
 
 def build_torch_binding() -> None:
     cflags, ldflags = torch_flags()
-    src = os.path.join(PKG, "torch", "csrc", "flash_train_torch.cpp")
-    obj = os.path.join(BUILD, "flash_train_torch.o")
-    run([HIPCC, *COMMON, *cflags, "-c", src, "-o", obj])
+    sources = ("flash_train_torch.cpp", "training.cpp")
+    objs = [os.path.join(BUILD, src + ".o") for src in sources]
+    with concurrent.futures.ThreadPoolExecutor(len(sources)) as pool:
+        list(pool.map(lambda s: run([HIPCC, *COMMON, *cflags, "-c", os.path.join(PKG, "torch", "csrc", s[0]), "-o", s[1]]),
+                      zip(sources, objs)))
     suffix = sysconfig.get_config_var("EXT_SUFFIX")
     out = os.path.join(PKG, "torch", "_flash_train_torch" + suffix)
-    run([HIPCC, "-shared", "-fPIC", obj, "-o", out, f"-L{PKG}", "-lflash_train", "-Wl,-rpath,$ORIGIN/..",
+    run([HIPCC, "-shared", "-fPIC", *objs, "-o", out, f"-L{PKG}", "-lflash_train", "-Wl,-rpath,$ORIGIN/..",
          *ldflags, f"-L{ROCM}/lib"])
 
 

@@ -13,7 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_bool, c_char_p, c_double, c_int, c_int32, c_int64, c_size_t, c_uint8, c_uint32
+from ctypes import POINTER, c_bool, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint8, c_uint32
 from ctypes import c_uint64, c_void_p
 from typing import Optional, Sequence
 
@@ -31,6 +31,7 @@ SUCCESS, INVALID_ARGUMENT, OUT_OF_MEMORY, OVERFLOW, UNSUPPORTED, INTERNAL_ERROR 
 STATUS_NAMES = {0: "SUCCESS", 1: "INVALID_ARGUMENT", 2: "OUT_OF_MEMORY", 3: "OVERFLOW", 4: "UNSUPPORTED",
                 50: "INTERNAL_ERROR"}
 FP64, INT64, UINT64, FP32, INT32, UINT32, FP16, BF16 = 1, 2, 3, 4, 5, 6, 7, 8
+UINT8 = 17
 NUMERIC_TYPE_COUNT = 24
 INDEX_INVALID, INDEX_CONTINUOUS, INDEX_SF_SWIZZLED, INDEX_GROUPED_CONTINUOUS = 0, 1, 2, 3
 INDEX_TYPE_COUNT = 4
@@ -49,10 +50,16 @@ EXPORTED_SYMBOLS = (
     "ftrainPlanGetPrimitiveRequiredWorkspaceBytes", "ftrainPlanExecutePrimitive",
     "ftrainGemm",
 )
-# The reference's 29 entry points plus ftrainGemmNoAlloc, which has no
-# reference counterpart (for callers that cannot allocate device memory).
+# The reference's 29 entry points plus those without a reference counterpart:
+# ftrainGemmNoAlloc (for callers that cannot allocate device memory) and the
+# operators around a training step's products.
 REFERENCE_SYMBOLS = EXPORTED_SYMBOLS
-EXPORTED_SYMBOLS = REFERENCE_SYMBOLS + ("ftrainGemmNoAlloc",)
+TRAINING_SYMBOLS = (
+    "ftrainLinearCrossEntropyWorkspaceBytes", "ftrainLinearCrossEntropy", "ftrainLinearCrossEntropyBackward",
+    "ftrainMoeRouteWorkspaceBytes", "ftrainMoeRoute", "ftrainMoeRouteBackward",
+    "ftrainClipGradNormWorkspaceBytes", "ftrainClipGradNorm",
+)
+EXPORTED_SYMBOLS = REFERENCE_SYMBOLS + ("ftrainGemmNoAlloc",) + TRAINING_SYMBOLS
 
 
 class StorageView(ctypes.Structure):
@@ -108,6 +115,15 @@ def _declare(lib: ctypes.CDLL) -> ctypes.CDLL:
         "ftrainPlanExecutePrimitive": (st, [_H, c_uint64, c_void_p, c_uint64, c_void_p]),
         "ftrainGemm": (st, [StorageView] * 6 + [c_uint8, c_void_p, c_uint64, c_void_p]),
         "ftrainGemmNoAlloc": (st, [StorageView] * 6 + [c_uint8, c_void_p]),
+        "ftrainLinearCrossEntropyWorkspaceBytes": (st, [StorageView] * 2 + [c_bool, POINTER(c_uint64)]),
+        "ftrainLinearCrossEntropy": (st, [StorageView] * 5 + [c_int64, c_void_p, c_uint64, c_void_p]),
+        "ftrainLinearCrossEntropyBackward": (st, [StorageView] * 7 + [c_int64, c_void_p, c_uint64, c_void_p]),
+        "ftrainMoeRouteWorkspaceBytes": (st, [StorageView, POINTER(c_uint64)]),
+        "ftrainMoeRoute": (st, [StorageView] * 8 + [c_bool, c_void_p, c_uint64, c_void_p]),
+        "ftrainMoeRouteBackward": (st, [StorageView] * 8 + [c_bool, c_void_p]),
+        "ftrainClipGradNormWorkspaceBytes": (st, [POINTER(c_uint64)]),
+        "ftrainClipGradNorm": (st, [POINTER(StorageView), POINTER(StorageView), c_uint32, StorageView, c_float, c_float,
+                                    c_void_p, c_uint64, c_void_p]),
     }
     for name, (res, args) in sigs.items():
         fn = getattr(lib, name)

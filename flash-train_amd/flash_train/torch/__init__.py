@@ -7,6 +7,13 @@ and optional c (m x n) fp32, rank-2, contiguous device tensors; d is
 allocated with ``torch.empty`` and computed on the current stream.
 RuntimeError on any violated check.
 
+Around a training step's products (include/flash_train/flash_train.h says
+what each computes; none has a counterpart in the reference):
+``linear_cross_entropy`` (an output head's loss, its logits never kept),
+``moe_route`` (a router's choice, gates, packed rows and balance loss), both
+differentiable and over their ``_forward`` and ``_backward`` calls, and
+``clip_grad_norm``.
+
 The native extension is required: importing this module without it raises
 (there is no CPU or eager fallback).
 """
@@ -20,7 +27,14 @@ _pkg = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 ctypes.CDLL(os.path.join(_pkg, "libflash_train.so"), mode=ctypes.RTLD_GLOBAL)
 
 try:
-    from ._flash_train_torch import gemm  # noqa: E402
+    from ._flash_train_torch import (  # noqa: E402
+        clip_grad_norm,
+        gemm,
+        linear_cross_entropy_backward,
+        linear_cross_entropy_forward,
+        moe_route_backward,
+        moe_route_forward,
+    )
 except ModuleNotFoundError as exc:  # pragma: no cover - build problem
     if exc.name != "flash_train.torch._flash_train_torch":
         raise
@@ -28,4 +42,15 @@ except ModuleNotFoundError as exc:  # pragma: no cover - build problem
         "flash_train.torch: the native extension is not built; run `python flash-train_amd/build.py`"
     ) from exc
 
-__all__ = ["gemm"]
+from .training import linear_cross_entropy, moe_route  # noqa: E402
+
+__all__ = [
+    "gemm",
+    "linear_cross_entropy",
+    "linear_cross_entropy_forward",
+    "linear_cross_entropy_backward",
+    "moe_route",
+    "moe_route_forward",
+    "moe_route_backward",
+    "clip_grad_norm",
+]

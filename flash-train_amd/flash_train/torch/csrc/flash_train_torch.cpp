@@ -3,14 +3,16 @@
 // Checks and defaults follow the reference binding
 // (python/flash_train/torch/csrc/flash_train_torch.cpp:34-75).  The stream is
 // torch's current HIP stream read natively (c10::hip::getCurrentHIPStreamMasqueradingAsCUDA),
-// not through a Python call as the reference does (:28-32), and the whole
-// binding is one translation unit.
+// not through a Python call as the reference does (:28-32).  The operators
+// around a training step's products are bound in training.cpp.
 #include <torch/extension.h>
 
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
 #include <flash_train/flash_train.h>
+
+#include "training.hpp"
 
 namespace {
 
@@ -66,4 +68,5 @@ PYBIND11_MODULE(_flash_train_torch, m) {
     m.doc() = "flash-train for MI355X PyTorch binding";
     m.def("gemm", &gemm, "d = alpha * (a @ b) + beta * c on the current stream", py::arg("a"), py::arg("b"),
           py::arg("c") = py::none(), py::arg("alpha") = 1.0, py::arg("beta") = 0.0);
+    bindTraining(m);
 }
