@@ -83,6 +83,9 @@ LIB_SOURCES = [
     "csrc/api/train_api.cpp",
     "csrc/train/clip.hip",
     "csrc/train/cross_entropy.hip",
+    "csrc/train/cross_entropy_bf16.hip",
+    "csrc/train/cross_entropy_fp16.hip",
+    "csrc/train/cross_entropy_fp32.hip",
     "csrc/train/route.hip",
 ]
 TESTING_SOURCES = ["csrc/api/testing_api.cpp"]

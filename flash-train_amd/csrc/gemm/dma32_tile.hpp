@@ -126,8 +126,21 @@ static __device__ __attribute__((aligned(256))) float dma32_dummy[512];
 // (n not a multiple of 4) is read from the row's last 4 columns instead, and the epilogue of a last
 // column tile, element by element, puts its values where they belong; a k tail's crossing chunks are
 // staged element by element.
-template <int BM, int BN, int WM, int WN, bool SPLIT, bool TB = false, bool TA = false, bool U = false>
-__device__ __forceinline__ void fp32_gemm_dma_tile(const GemmParams& p, int bid, int z, int band = 4) {
+//
+// END: what is made of the finished tile.  StoreTile, d = alpha acc + beta c, or a functor that another
+// operator calls the tile with: end(row, column, v, inside, left) gets 4 adjacent sums v of one row (16
+// adjacent lanes hold 64 adjacent columns of it, and every lane of the wave calls it); inside: the row
+// lies in the matrix; left: how many columns from `column` on do.
+// read_m, read_n: rows and columns that a's and b's storage holds, where that is more than m and n (a
+// transposed operand is read in whole chunks of 4); 0: m, n.
+// FOLD: the sums of every FOLD stages of 32 k are kept apart and then added to the total, so the error of
+// a long k grows with the roots of both counts instead of that of k.
+struct StoreTile {};
+
+template <int BM, int BN, int WM, int WN, bool SPLIT, bool TB = false, bool TA = false, bool U = false,
+          class END = StoreTile, int FOLD = 0>
+__device__ __forceinline__ void fp32_gemm_dma_tile(const GemmParams& p, int bid, int z, int band = 4, const END& end = END{},
+                                                   int read_m = 0, int read_n = 0) {
     static_assert(WM * WN == 4, "4 waves");
     constexpr int WTM = BM / WM, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16, NC = TN / 4;
     static_assert(TN % 4 == 0 && TM >= 1, "column runs of four blocks");
@@ -157,6 +170,7 @@ __device__ __forceinline__ void fp32_gemm_dma_tile(const GemmParams& p, int bid,
     tile_of(bid, p.tiles_m, p.tiles_n, tm, tn, band);
     const int m0 = tm * BM, n0 = tn * BN;
     const int M = p.m, N = p.n;
+    const int MX = read_m > 0 ? read_m : M, NX = read_n > 0 ? read_n : N;
     const int kbeg = SPLIT ? z * p.k_chunk : 0;
     const int kend = SPLIT ? min(p.k, kbeg + p.k_chunk) : p.k;
     // Whole stages go through the DMA pipeline; a partial last one (k_tail) is staged afterwards.
@@ -175,7 +189,7 @@ __device__ __forceinline__ void fp32_gemm_dma_tile(const GemmParams& p, int bid,
     // stored); 255 rows of lda < 2^22 keep the lane offset below 2^32.
     const unsigned ar     = 8 * wave + (lane >> 3);
     const unsigned achunk = 16 * ((lane & 7) ^ a_swz(ar));
-    const unsigned alast  = static_cast<unsigned>(min(M - 1 - m0, BM - 1));
+    const unsigned alast  = static_cast<unsigned>(min(MX - 1 - m0, BM - 1));
     const unsigned lda4   = static_cast<unsigned>(4 * lda);
     const char* abase_r   = reinterpret_cast<const char*>(p.a + (size_t)m0 * lda_r + kbeg);
     const char* abase     = none ? dummy : abase_r;
@@ -183,12 +197,12 @@ __device__ __forceinline__ void fp32_gemm_dma_tile(const GemmParams& p, int bid,
     // lane % CPR holds chunk (lane % CPR) ^ swizzle; a chunk past n, or across it, is clamped onto the
     // last 4 columns (n >= 4; nb is the leftmost column read).  x = the swizzle bit of the block's k
     // rows.
-    const int nb        = U ? min(n0, N - 4) : n0;
+    const int nb        = U ? min(n0, NX - 4) : n0;
     const char* bbase_r = reinterpret_cast<const char*>(p.b + (size_t)kbeg * ldb_r + nb);
     const char* bbase   = none ? dummy : bbase_r;
     auto boff = [&](int x, int64_t ld) {
         const int kr = lane / CPR, chunk = (lane % CPR) ^ (x ? 16 : 0);
-        return static_cast<unsigned>((kr * ld + (min(n0 + 4 * chunk, N - 4) - nb)) * 4);
+        return static_cast<unsigned>((kr * ld + (min(n0 + 4 * chunk, NX - 4) - nb)) * 4);
     };
     const unsigned boff0 = boff(0, ldb), boff1 = BSWZ ? boff(1, ldb) : boff0;
     // Column-major a: block q = wave + 4 j holds k rows RA q .. RA q + RA - 1 of the stage (lane: k
@@ -198,7 +212,7 @@ __device__ __forceinline__ void fp32_gemm_dma_tile(const GemmParams& p, int bid,
     const char* atbase   = none ? dummy : atbase_r;
     auto aoff = [&](int x, int64_t ld) {
         const int kr = lane / CPA, chunk = (lane % CPA) ^ (x ? 16 : 0);
-        return static_cast<unsigned>((kr * ld + (min(m0 + 4 * chunk, M - 4) - m0)) * 4);
+        return static_cast<unsigned>((kr * ld + (min(m0 + 4 * chunk, MX - 4) - m0)) * 4);
     };
     const unsigned aoff0 = TA ? aoff(0, lda) : 0u, aoff1 = TA && ASWZ ? aoff(1, lda) : aoff0;
     auto dma_a = [&](int st, int j, unsigned lds) {
@@ -220,7 +234,7 @@ __device__ __forceinline__ void fp32_gemm_dma_tile(const GemmParams& p, int bid,
     // 255 columns of ldb < 2^22 keep the lane offset below 2^32.
     const char* btbase_r = reinterpret_cast<const char*>(p.b + (size_t)n0 * ldb_r + kbeg);
     const char* btbase   = none ? dummy : btbase_r;
-    const unsigned blast = static_cast<unsigned>(min(N - 1 - n0, BN - 1));
+    const unsigned blast = static_cast<unsigned>(min(NX - 1 - n0, BN - 1));
     auto dma_bt = [&](int st, int j, unsigned lds) {
         const int q = wave + 4 * j, t = (lane & 7) ^ (q & 7);
         const int cb = 4 * ((lane >> 3) & 1) + 2 * (lane >> 5) + (t & 1), ch = 4 * (t >> 2) + 2 * ((lane >> 4) & 1) + ((t >> 1) & 1);
@@ -286,6 +300,26 @@ __device__ __forceinline__ void fp32_gemm_dma_tile(const GemmParams& p, int bid,
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+
+    static_assert(FOLD % 2 == 0, "the stage loop takes two at a time");
+    floatx4 total[FOLD > 0 ? TM : 1][FOLD > 0 ? TN : 1];
+    if constexpr (FOLD > 0) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) total[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+    auto fold = [&] {
+        if constexpr (FOLD > 0) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) {
+                    total[i][j] += acc[i][j];
+                    acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+                }
+        }
+    };
 
     // Operands of one half stage: fa[bi] (4 k-steps), fb[s][cc] (4 columns); column-major b:
     // fb[bj & 3][bj >> 2] holds block bj's 4 k-steps.
@@ -374,6 +408,8 @@ __device__ __forceinline__ void fp32_gemm_dma_tile(const GemmParams& p, int bid,
         for (; st + 1 < nst; st += 2) {
             FT_DMA32_PHASE(As0, Bs0, As1, Bs1, la0, lb0, st)
             FT_DMA32_PHASE(As1, Bs1, As0, Bs0, la1, lb1, st + 1)
+            if constexpr (FOLD > 0)
+                if (st % FOLD == FOLD - 2) fold();
         }
         if (st < nst) {
             FT_DMA32_PHASE(As0, Bs0, As1, Bs1, la0, lb0, st)
@@ -389,11 +425,12 @@ __device__ __forceinline__ void fp32_gemm_dma_tile(const GemmParams& p, int bid,
         if (k_tail > 0) {
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
             // left: how many of the chunk's elements lie before kend (only a k-contiguous chunk of an
-            // unaligned tile can hold some of both kinds).
+            // unaligned tile, or of storage padded to whole chunks with zeros, can hold some of both
+            // kinds; the second is read whole).
             typedef float floatx4u __attribute__((ext_vector_type(4), aligned(4)));
             auto put = [&](float* stage, int q, int left, const char* src) {
                 floatx4 v = floatx4{0.f, 0.f, 0.f, 0.f};
-                if (left >= 4) {
+                if (left >= (U ? 4 : 1)) {
                     v = U ? *reinterpret_cast<const floatx4u*>(src) : *reinterpret_cast<const floatx4*>(src);
                 } else if (U && left > 0) {
                     const float* e = reinterpret_cast<const float*>(src);
@@ -438,6 +475,31 @@ __device__ __forceinline__ void fp32_gemm_dma_tile(const GemmParams& p, int bid,
             rotate();
             run_half(fa0, fb0, fa1, fb1, As0, Bs0, 0, std::false_type{}, 0, 0u, 0u);
         }
+    }
+
+    if constexpr (FOLD > 0) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] += total[i][j];
+    }
+    if constexpr (!std::is_same_v<END, StoreTile>) {
+        const int rows_left = M - m0;
+#pragma unroll
+        for (int bi = 0; bi < TM; ++bi)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int row = TA ? wrow + (bi >> 2) * 64 + 16 * g + 4 * r + (bi & 3) : wrow + 16 * bi + 4 * g + r;
+#pragma unroll
+                for (int q = 0; q < NC; ++q) {
+                    const int col = wcol + 64 * q + 4 * j16;
+                    float out[4];
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) out[t] = acc[bi][4 * q + t][r];
+                    end(m0 + row, n0 + col, out, row < rows_left, N - n0 - col);
+                }
+            }
+        return;
     }
 
     // Epilogue, one row block at a time: block (bi, bj) register r is D[row 16 bi + 4 g + r][col

@@ -199,8 +199,18 @@ struct Operand {
 // on it with a leading dimension of 0 keep every lane's offset within 512 bytes.
 static __device__ __attribute__((aligned(256))) u16 pp_dummy[512];
 
-template <bool BF16, bool TA, bool TB>
-__device__ __forceinline__ void half_gemm_pp_tile(const HalfGemmParams& p, int bid, int band) {
+// The plain product's end of a tile: d = alpha acc + beta c.
+struct StoreTile {};
+
+// END: what is made of the finished tile.  StoreTile, or a functor that another operator calls the tile
+// with: end(row, column, v, inside, left) gets 8 adjacent sums v of one row (a row's 256 columns are 32
+// lanes' in order, the two halves of a wave hold adjacent rows, and every lane of the wave calls it);
+// inside: the row lies in the matrix; left: how many columns from `column` on do.
+// read_m, read_n: rows and columns that a's and b's storage holds, where that is more than m and n (a
+// transposed operand is read in whole chunks of 8); 0: m, n.
+template <bool BF16, bool TA, bool TB, class END = StoreTile>
+__device__ __forceinline__ void half_gemm_pp_tile(const HalfGemmParams& p, int bid, int band, const END& end = END{},
+                                                  int read_m = 0, int read_n = 0) {
     constexpr bool A_TR = TA, B_TR = !TB;
     __shared__ __attribute__((aligned(1024))) char lds[3 * kShortStage];
     const int tid = threadIdx.x, lane = tid & 63, j16 = lane & 15, g = lane >> 4;
@@ -210,6 +220,7 @@ __device__ __forceinline__ void half_gemm_pp_tile(const HalfGemmParams& p, int b
     tile_of(bid, p.tiles_m, p.tiles_n, tm, tn, band);
     const int m0 = tm * 256, n0 = tn * 256;
     const int M = p.m, N = p.n;
+    const int MX = read_m > 0 ? read_m : M, NX = read_n > 0 ? read_n : N;
     const int nst = p.k / kStageK, k_tail = p.k - nst * kStageK;
 
     const u16* const pa = static_cast<const u16*>(p.a);
@@ -217,8 +228,8 @@ __device__ __forceinline__ void half_gemm_pp_tile(const HalfGemmParams& p, int b
     Operand<A_TR> opa;
     Operand<B_TR> opb;
     if (nst > 0) {
-        opa.init(pa, p.lda, m0, M, wave, lane);
-        opb.init(pb, p.ldb, n0, N, wave, lane);
+        opa.init(pa, p.lda, m0, MX, wave, lane);
+        opb.init(pb, p.ldb, n0, NX, wave, lane);
     } else {
         opa.init(pp_dummy, 0, 0, 256, wave, lane);
         opb.init(pp_dummy, 0, 0, 256, wave, lane);
@@ -400,8 +411,8 @@ __device__ __forceinline__ void half_gemm_pp_tile(const HalfGemmParams& p, int b
     // k tail: the partial last stage is staged by ordinary loads (zeros past k), then multiplied.
     if (k_tail > 0) {
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        opa.init(pa, p.lda, m0, M, wave, lane);
-        opb.init(pb, p.ldb, n0, N, wave, lane);
+        opa.init(pa, p.lda, m0, MX, wave, lane);
+        opb.init(pb, p.ldb, n0, NX, wave, lane);
         const char* const ta = opa.base + (size_t)nst * opa.step;
         const char* const tb = opb.base + (size_t)nst * opb.step;
         opa.fill(ta, 0, lds + kA0, wave, lane, k_tail);
@@ -417,6 +428,38 @@ __device__ __forceinline__ void half_gemm_pp_tile(const HalfGemmParams& p, int b
             matrix(acc[i][0], f0);
             matrix(acc[i][1], f1);
         }
+    }
+
+    if constexpr (!std::is_same_v<END, StoreTile>) {
+        // The epilogue's turn through LDS (below), two rows of 512 bytes to an access.
+        const int rows_left = M - m0, er = lane >> 5, ec = 8 * (lane & 31);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (128 * i >= rows_left) break;
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int v = 0; v < 2; ++v)
+                        *reinterpret_cast<floatx4*>(lds + (64 * wm + 16 * u + j16) * 1024 +
+                                                    16 * ((32 * j + 8 * wn + 4 * v + g) ^ j16)) = acc[i][j][u][v];
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+                const int r = 16 * wave + 2 * t + er, row = 128 * i + r;
+                float out[8];
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const floatx4 f = *reinterpret_cast<const floatx4*>(lds + r * 1024 + 16 * ((ec / 4 + q) ^ (r & 15)));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) out[4 * q + e] = f[e];
+                }
+                end(m0 + row, n0 + ec, out, row < rows_left, N - n0 - ec);
+            }
+        }
+        return;
     }
 
     // Epilogue.  Lane (j16, g) holds row j16, columns 4 g .. 4 g + 3 of every 16x16 block; stored from

@@ -13,6 +13,7 @@
 // and gradients NaN.
 #include <algorithm>
 
+#include "cross_entropy.hpp"
 #include "device.hpp"
 #include "ft/train.hpp"
 
@@ -21,20 +22,6 @@ namespace {
 
 constexpr int kThreads     = 256;
 constexpr int kPackThreads = 1024;
-
-// What the device knows of the batch.
-struct Head {
-    int32_t valid;    // packed rows
-    float scale;      // dl is kept times this power of two
-    float inv_scale;
-};
-
-// One packed row: where its gradient of the loss, its lse and its target are.
-struct RowInfo {
-    float lse;
-    float grad;      // times Head::scale
-    int32_t target;  // -1: outside the classes
-};
 
 struct PackArgs {
     const void* target;
@@ -119,95 +106,6 @@ __global__ __launch_bounds__(kThreads) void copyRows(const T* src, int64_t src_l
     }
 }
 
-enum class Mode { kLogSum, kGradLogits, kGradHidden, kGradWeight };
-
-struct TileArgs {
-    const void *a, *b;  // element (i, k) of a at i a_row + k a_col, (k, j) of b at k b_row + j b_col
-    int64_t a_row, a_col, b_row, b_col;
-    int32_t m, n, k;
-    const Head* head;
-    const RowInfo* rows;
-    int32_t first_class;
-    float2* part;  // kLogSum: of each row, each tile column's maximum and sum
-    float* hit;    // kLogSum: each row's logit of its target
-    int32_t parts;
-    void* d;
-    int64_t ldd;
-    int32_t padded;  // kGradLogits: columns to write (zeros past n)
-    bool add;        // kGradHidden
-};
-
-// A 64x64 tile of a @ b by 256 threads, 4x4 outputs each, and what the mode makes of it.
-template <class T, Mode MODE>
-__global__ __launch_bounds__(kThreads) void tile(TileArgs p) {
-    constexpr int S = 64, K = 16;
-    __shared__ float As[K][S + 4], Bs[K][S + 4];
-    const int valid = p.head->valid;
-    const int M = MODE == Mode::kGradWeight ? p.m : min(p.m, valid), N = p.n;
-    const int D = MODE == Mode::kGradWeight ? min(p.k, valid) : p.k;
-    const int m0 = blockIdx.y * S, n0 = blockIdx.x * S;
-    if (m0 >= M) return;
-    const int tr = threadIdx.x / 16, tc = threadIdx.x % 16;
-    const T* const a = static_cast<const T*>(p.a);
-    const T* const b = static_cast<const T*>(p.b);
-    float acc[4][4] = {};
-    for (int k0 = 0; k0 < D; k0 += K) {
-        for (int i = threadIdx.x; i < S * K; i += kThreads) {
-            const int ak = p.a_col == 1 ? i % K : i / S, am = p.a_col == 1 ? i / K : i % S;
-            As[ak][am] = m0 + am < M && k0 + ak < D ? toFloat(a[(m0 + am) * p.a_row + (k0 + ak) * p.a_col]) : 0.f;
-            const int bk = p.b_row == 1 ? i % K : i / S, bn = p.b_row == 1 ? i / K : i % S;
-            Bs[bk][bn] = n0 + bn < N && k0 + bk < D ? toFloat(b[(k0 + bk) * p.b_row + (n0 + bn) * p.b_col]) : 0.f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(As[k][4 * tr + i], Bs[k][4 * tc + j], acc[i][j]);
-        __syncthreads();
-    }
-    for (int i = 0; i < 4; ++i) {
-        const int row = m0 + 4 * tr + i;
-        if constexpr (MODE == Mode::kLogSum) {
-            float top = -INFINITY, sum = 0.f;
-            const int y = row < M ? p.rows[row].target - p.first_class : -1;
-            for (int j = 0; j < 4; ++j) {
-                const int col = n0 + 4 * tc + j;
-                if (col < N) top = fmaxf(top, acc[i][j]);
-                if (row < M && col < N && col == y) p.hit[row] = acc[i][j];
-            }
-            top = groupMax<16>(top);
-            for (int j = 0; j < 4; ++j)
-                if (n0 + 4 * tc + j < N) sum += expf(acc[i][j] - top);
-            sum = groupSum<16>(sum);
-            if (tc == 0 && row < M)
-                p.part[static_cast<int64_t>(row) * p.parts + p.first_class / S + blockIdx.x] = make_float2(top, sum);
-        } else if (row < M) {
-            for (int j = 0; j < 4; ++j) {
-                const int col = n0 + 4 * tc + j;
-                if constexpr (MODE == Mode::kGradLogits) {
-                    if (col >= p.padded) continue;
-                    const RowInfo r = p.rows[row];
-                    float v         = 0.f;
-                    if (col < N) {
-                        v = expf(acc[i][j] - r.lse) - (col == r.target - p.first_class ? 1.f : 0.f);
-                        v = r.target < 0 ? NAN : v * r.grad;
-                    }
-                    static_cast<T*>(p.d)[row * p.ldd + col] = static_cast<T>(v);
-                } else if (col < N) {
-                    if constexpr (MODE == Mode::kGradHidden) {
-                        float* const d = static_cast<float*>(p.d) + row * p.ldd + col;
-                        *d             = p.add ? *d + acc[i][j] : acc[i][j];
-                    } else {
-                        static_cast<T*>(p.d)[row * p.ldd + col] = static_cast<T>(acc[i][j] * p.head->inv_scale);
-                    }
-                }
-            }
-        }
-    }
-}
-
 // loss and lse of every kept token from its tiles' maxima and sums; a wave per token.
 __global__ __launch_bounds__(kThreads) void finishLoss(const float2* part, const float* hit, const RowInfo* rows,
                                                        const int32_t* place, int64_t tokens, int parts, float* loss,
@@ -239,34 +137,60 @@ __global__ __launch_bounds__(kThreads) void finishLoss(const float2* part, const
 template <class T>
 __global__ __launch_bounds__(kThreads) void finishHidden(const float* sums, int64_t ld, const int32_t* place,
                                                          const Head* head, T* out, int64_t out_ld, int64_t tokens,
-                                                         int64_t cols) {
+                                                         int64_t cols, int slices, int64_t slice) {
     const float inv = head->inv_scale;
     for (int64_t t = blockIdx.x; t < tokens; t += gridDim.x) {
         const int row           = place[t];
         const float* const from = sums + static_cast<int64_t>(row) * ld;
-        for (int64_t i = threadIdx.x; i < cols; i += kThreads)
-            out[t * out_ld + i] = static_cast<T>(row < 0 ? 0.f : from[i] * inv);
+        for (int64_t i = threadIdx.x * 4; i < cols; i += kThreads * 4) {
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (row >= 0) {
+                for (int z = 0; z < slices; ++z) {
+                    const float4 x = *reinterpret_cast<const float4*>(from + z * slice + i);
+                    v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+                }
+            }
+            T* const to = out + t * out_ld + i;
+            to[0]       = static_cast<T>(v.x * inv);
+            if (i + 1 < cols) to[1] = static_cast<T>(v.y * inv);
+            if (i + 2 < cols) to[2] = static_cast<T>(v.z * inv);
+            if (i + 3 < cols) to[3] = static_cast<T>(v.w * inv);
+        }
     }
 }
 
 uint64_t ceilDiv(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 uint64_t roundUp(uint64_t a, uint64_t b) { return ceilDiv(a, b) * b; }
 
+// Bytes of a piece of dl: the last-level cache's 256 MiB, which it is read from twice.
+constexpr uint64_t kPieceBytes = 256ull << 20;
+// Workgroups that fill the device's 256 CUs.
+constexpr uint64_t kFill = 256;
+
 // The workspace, laid out for one call.
 struct Layout {
     uint64_t bytes = 0;
-    uint64_t head, place, rows, x, part, hit, dl, dx;
-    int64_t padded;  // columns of a packed row of x
+    uint64_t head, place, rows, x, w, part, hit, dl, dx;
+    int64_t padded;  // columns of a packed row of x (and w)
     int64_t piece;   // classes of one piece
     int64_t parts;
+    int slices;      // of a piece's classes, each with sums of its own for dx
+    int64_t slice;   // elements of one slice's sums
+    bool pack_w;     // the weight's rows are not whole 16-byte units: each piece is copied first
 
     Layout(const CrossEntropy& p, bool backward) {
         const uint64_t tokens = p.hidden.rows, hidden = p.hidden.cols, classes = p.weight.rows;
-        const uint64_t size = elementBytes(p.type);
-        padded              = roundUp(hidden, 16 / size);
-        piece               = std::min<int64_t>(roundUp(classes, 64), 8192);
-        parts               = ceilDiv(classes, 64);
-        auto take           = [&](uint64_t n) {
+        const uint64_t size = elementBytes(p.type), unit = 16 / size;
+        padded = roundUp(hidden, unit);
+        pack_w = hidden % unit != 0 || p.weight.ld % unit != 0 || reinterpret_cast<uintptr_t>(p.weight.data) % 16 != 0;
+        const uint64_t row = backward ? tokens * size : pack_w ? padded * size : 1;
+        piece = std::min(std::max<uint64_t>(kPieceBytes / std::max<uint64_t>(row, 1) / 256 * 256, 2048), roundUp(classes, 256));
+        parts = ceilDiv(classes, headPartClasses(p.type));
+        const uint64_t tile  = p.type == FTRAIN_NUMERIC_TYPE_FP32 ? 128 : 256;
+        const uint64_t tiles = std::max<uint64_t>(1, ceilDiv(tokens, tile) * ceilDiv(hidden, tile));
+        slices               = static_cast<int>(std::max<uint64_t>(1, std::min(kFill / tiles, static_cast<uint64_t>(piece) / 512)));
+        slice                = tokens * padded;
+        auto take            = [&](uint64_t n) {
             const uint64_t at = bytes;
             bytes += roundUp(n, 256);
             return at;
@@ -275,10 +199,11 @@ struct Layout {
         place = take(tokens * 4);
         rows  = take(tokens * sizeof(RowInfo));
         x     = take(tokens * padded * size);
+        w     = pack_w ? take(piece * padded * size) : 0;
         part  = backward ? 0 : take(tokens * parts * sizeof(float2));
         hit   = backward ? 0 : take(tokens * 4);
         dl    = backward ? take(tokens * piece * size) : 0;
-        dx    = backward ? take(tokens * padded * 4) : 0;
+        dx    = backward ? take(slices * slice * 4) : 0;
     }
 };
 
@@ -303,20 +228,36 @@ Buffers packInputs(const CrossEntropy& p, const Layout& l, char* base, bool back
     return b;
 }
 
-dim3 gridOf(int64_t m, int64_t n) { return dim3(static_cast<uint32_t>(ceilDiv(n, 64)), static_cast<uint32_t>(ceilDiv(m, 64))); }
+// The classes from `first` on, `n` of them, in rows of whole 16-byte units.
+template <class T>
+const T* weightPiece(const CrossEntropy& p, const Layout& l, char* base, int64_t first, int64_t n, int64_t& ld,
+                     hipStream_t stream) {
+    const T* const from = static_cast<const T*>(p.weight.data) + first * p.weight.ld;
+    ld                  = p.weight.ld;
+    if (!l.pack_w) return from;
+    T* const to = reinterpret_cast<T*>(base + l.w);
+    launch(&copyRows<T>, "cross entropy weight copy", dim3(static_cast<uint32_t>(std::min<int64_t>(n, 65536))), dim3(kThreads),
+           stream, from, p.weight.ld, n, p.weight.cols, to, l.padded, l.padded, static_cast<const int32_t*>(nullptr));
+    ld = l.padded;
+    return to;
+}
 
 template <class T>
 void forward(const CrossEntropy& p, char* base, hipStream_t stream) {
     const Layout l(p, false);
     const Buffers b = packInputs<T>(p, l, base, false, stream);
-    TileArgs t{};
-    t.a = base + l.x, t.a_row = l.padded, t.a_col = 1;
-    t.b = p.weight.data, t.b_row = 1, t.b_col = p.weight.ld;
-    t.m = p.hidden.rows, t.n = p.weight.rows, t.k = p.hidden.cols;
+    HeadTileArgs t{};
+    t.a = base + l.x, t.lda = l.padded;
+    t.m = p.hidden.rows, t.k = l.padded;
     t.head = b.head, t.rows = b.rows;
     t.part = reinterpret_cast<float2*>(base + l.part), t.hit = reinterpret_cast<float*>(base + l.hit);
-    t.parts = l.parts;
-    launch(&tile<T, Mode::kLogSum>, "cross entropy logits", gridOf(t.m, t.n), dim3(kThreads), stream, t);
+    t.parts              = l.parts;
+    const int64_t classes = p.weight.rows, piece = l.pack_w ? l.piece : classes;
+    for (int64_t v = 0; v < classes; v += piece) {
+        t.n = std::min(piece, classes - v), t.first_class = v;
+        t.b = weightPiece<T>(p, l, base, v, t.n, t.ldb, stream);
+        launchHeadTile(p.type, HeadTile::kLogSum, t, 1, stream);
+    }
     launch(&finishLoss, "cross entropy loss", dim3(static_cast<uint32_t>(ceilDiv(p.hidden.rows, kThreads / kWave))),
            dim3(kThreads), stream, static_cast<const float2*>(t.part), static_cast<const float*>(t.hit),
            static_cast<const RowInfo*>(b.rows), static_cast<const int32_t*>(b.place), p.hidden.rows,
@@ -328,34 +269,57 @@ void backward(const CrossEntropy& p, char* base, hipStream_t stream) {
     const Layout l(p, true);
     const Buffers b = packInputs<T>(p, l, base, true, stream);
     const int64_t tokens = p.hidden.rows, hidden = p.hidden.cols, classes = p.weight.rows;
+    const int64_t unit = 16 / sizeof(T);
     for (int64_t v = 0; v < classes; v += l.piece) {
-        const int64_t n  = std::min(l.piece, classes - v);
-        const T* const w = static_cast<const T*>(p.weight.data) + v * p.weight.ld;
-        TileArgs t{};
+        HeadTileArgs t{};
         t.head = b.head, t.rows = b.rows, t.first_class = v;
-        t.a = base + l.x, t.a_row = l.padded, t.a_col = 1;
-        t.b = w, t.b_row = 1, t.b_col = p.weight.ld;
-        t.m = tokens, t.n = n, t.k = hidden;
-        t.d = base + l.dl, t.ldd = l.piece, t.padded = n;
-        if (tokens > 0) launch(&tile<T, Mode::kGradLogits>, "cross entropy logits' gradient", gridOf(tokens, n), dim3(kThreads), stream, t);
-        t.a = base + l.dl, t.a_row = l.piece, t.a_col = 1;
-        t.b = w, t.b_row = p.weight.ld, t.b_col = 1;
-        t.n = hidden, t.k = n;
-        t.d = base + l.dx, t.ldd = l.padded, t.add = v > 0;
-        if (tokens > 0) launch(&tile<T, Mode::kGradHidden>, "cross entropy hidden gradient", gridOf(tokens, hidden), dim3(kThreads), stream, t);
-        t.a_row = 1, t.a_col = l.piece;
-        t.b = base + l.x, t.b_row = l.padded, t.b_col = 1;
-        t.m = n, t.n = hidden, t.k = tokens;
+        const int64_t n = std::min(l.piece, classes - v);
+        int64_t ldw;
+        const T* const w = weightPiece<T>(p, l, base, v, n, ldw, stream);
+        if (tokens > 0) {
+            t.a = base + l.x, t.lda = l.padded;
+            t.b = w, t.ldb = ldw;
+            t.d = base + l.dl, t.ldd = l.piece;
+            t.m = tokens, t.n = n, t.k = l.padded;
+            launchHeadTile(p.type, HeadTile::kGradLogits, t, 1, stream);
+            t.a = base + l.dl, t.lda = l.piece;
+            t.d = base + l.dx, t.ldd = l.padded;
+            t.n = l.padded, t.k = n;
+            // Whole stages of the tile to a slice; a last piece's slices may be fewer, its sums then
+            // leave the others as they are.
+            t.k_chunk        = roundUp(ceilDiv(n, l.slices), 64);
+            t.slice          = l.slice;
+            t.add            = v > 0;
+            const int slices = t.add ? static_cast<int>(ceilDiv(n, t.k_chunk)) : l.slices;
+            launchHeadTile(p.type, HeadTile::kGradHidden, t, slices, stream);
+        }
+        t.a = base + l.dl, t.lda = l.piece;
+        t.b = base + l.x, t.ldb = l.padded;
         t.d = static_cast<T*>(p.grad_weight.data) + v * p.grad_weight.ld, t.ldd = p.grad_weight.ld;
-        launch(&tile<T, Mode::kGradWeight>, "cross entropy weight gradient", gridOf(n, hidden), dim3(kThreads), stream, t);
+        t.m = n, t.n = hidden, t.k = tokens;
+        t.read_m = roundUp(n, unit), t.read_n = l.padded;
+        launchHeadTile(p.type, HeadTile::kGradWeight, t, 1, stream);
     }
-    if (tokens > 0) launch(&finishHidden<T>, "cross entropy hidden gradient's rows", dim3(static_cast<uint32_t>(std::min<int64_t>(tokens, 65536))),
-           dim3(kThreads), stream, reinterpret_cast<const float*>(base + l.dx), l.padded,
-           static_cast<const int32_t*>(b.place), static_cast<const Head*>(b.head), static_cast<T*>(p.grad_hidden.data),
-           p.grad_hidden.ld, tokens, hidden);
+    if (tokens > 0)
+        launch(&finishHidden<T>, "cross entropy hidden gradient's rows",
+               dim3(static_cast<uint32_t>(std::min<int64_t>(tokens, 65536))), dim3(kThreads), stream,
+               reinterpret_cast<const float*>(base + l.dx), l.padded, static_cast<const int32_t*>(b.place),
+               static_cast<const Head*>(b.head), static_cast<T*>(p.grad_hidden.data), p.grad_hidden.ld, tokens, hidden,
+               l.slices, l.slice);
 }
 
 }  // namespace
+
+int headPartClasses(FTrainNumericType type) { return type == FTRAIN_NUMERIC_TYPE_FP32 ? 64 : 256; }
+
+void launchHeadTile(FTrainNumericType type, HeadTile what, const HeadTileArgs& args, int slices, hipStream_t stream) {
+    if (type == FTRAIN_NUMERIC_TYPE_FP32)
+        launchHeadTileFp32(what, args, slices, stream);
+    else if (type == FTRAIN_NUMERIC_TYPE_BF16)
+        launchHeadTileBf16(what, args, slices, stream);
+    else
+        launchHeadTileFp16(what, args, slices, stream);
+}
 
 uint64_t crossEntropyWorkspace(const CrossEntropy& p, bool backward) { return Layout(p, backward).bytes; }
 

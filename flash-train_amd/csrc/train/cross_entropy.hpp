@@ -1,0 +1,64 @@
+// What the cross entropy's host code (cross_entropy.hip) and its tile kernels (one translation unit per
+// element type, cross_entropy_tiles.hpp) share.
+#pragma once
+
+#include <cstdint>
+
+#include <hip/hip_runtime.h>
+
+#include <flash_train/common.h>
+
+namespace ftrain::train {
+
+// What the device knows of the batch.
+struct Head {
+    int32_t valid;  // packed rows
+    float scale;    // dl is kept times this power of two
+    float inv_scale;
+};
+
+// One packed row: where its lse, its gradient of the loss and its target are.
+struct RowInfo {
+    float lse;
+    float grad;      // times Head::scale
+    int32_t target;  // -1: outside the classes
+};
+
+// The products of the two passes.
+enum class HeadTile {
+    kLogSum,      // tokens x classes: each row's maximum and sum of exponentials over a tile's classes
+    kGradLogits,  // tokens x classes: dl
+    kGradHidden,  // tokens x hidden = dl w, fp32 sums of a slice of the classes
+    kGradWeight,  // classes x hidden = dl^T x
+};
+
+struct HeadTileArgs {
+    const void *a, *b;
+    void* d;
+    int64_t lda, ldb, ldd;
+    int32_t m, n, k;
+    int32_t read_m, read_n;  // what the storage of transposed operands holds; 0: m, n
+    const Head* head;
+    const RowInfo* rows;
+    int32_t first_class;
+    // kLogSum: of each row, `parts` pairs of maximum and sum, and the logit of its target.
+    float2* part;
+    float* hit;
+    int32_t parts;
+    // kGradHidden: the classes of one of gridDim.z slices, elements from one slice's sums to the next's,
+    // and whether the sums of earlier classes are added to.
+    int32_t k_chunk;
+    int64_t slice;
+    bool add;
+};
+
+// Classes whose maximum and sum one tile leaves in one pair.
+int headPartClasses(FTrainNumericType type);
+// Launches the product; m counts every token, the kernels take the packed ones only.
+void launchHeadTile(FTrainNumericType type, HeadTile what, const HeadTileArgs& args, int slices, hipStream_t stream);
+
+void launchHeadTileFp32(HeadTile what, const HeadTileArgs& args, int slices, hipStream_t stream);
+void launchHeadTileBf16(HeadTile what, const HeadTileArgs& args, int slices, hipStream_t stream);
+void launchHeadTileFp16(HeadTile what, const HeadTileArgs& args, int slices, hipStream_t stream);
+
+}  // namespace ftrain::train
