@@ -209,9 +209,18 @@ static __device__ __attribute__((aligned(256))) u16 dma_dummy[512];
 // BM: tile rows (T by default; 64 with T = 128 for m of at most 64, row-major a only).
 // NB: stage buffers; a stage's DMAs run NB - 1 stages ahead of its use.
 // ROTATE: neighbouring column tiles start at different stages (the kernel below says why).
-template <bool BF16, bool TA, bool TB, int T = 128, bool SPLIT = false, int BM = T, int NB = 2, bool ROTATE = false>
+// END: what is made of the finished tile.  StoreTile, d = alpha acc + beta c, or a functor that another
+// operator calls the tile with: end(acc, a, b, m0, n0) gets the sums as the MFMAs leave them (above), the
+// workgroup's LDS of both operands (NB stages each), free once the workgroup has met at a barrier, and
+// the tile's first row and column.
+struct StoreTile {};
+template <bool BF16, bool TA, bool TB, int T = 128, bool SPLIT = false, int BM = T, int NB = 2, bool ROTATE = false,
+          class END = StoreTile>
 // band: tile rows per band of the tile order (tile_of).
-__device__ __forceinline__ void half_gemm_dma_tile(const HalfGemmParams& p, int bid, int z = 0, int band = 8) {
+// read_m, read_n: rows and columns that a's and b's storage holds, where that is more than m and n (a
+// transposed operand is read in whole chunks of 8); 0: m, n.
+__device__ __forceinline__ void half_gemm_dma_tile(const HalfGemmParams& p, int bid, int z = 0, int band = 8,
+                                                   const END& end = END{}, int read_m = 0, int read_n = 0) {
     constexpr bool A_TR = TA, B_TR = !TB;
     static_assert(BM == T || (BM == 64 && !TA), "64-row tiles take row-major a");
     constexpr int NBM = BM / 64, NBN = T / 64;  // 32x32 blocks per wave row / column
@@ -226,6 +235,7 @@ __device__ __forceinline__ void half_gemm_dma_tile(const HalfGemmParams& p, int 
     tile_of(bid, p.tiles_m, p.tiles_n, tm, tn, band);
     const int m0 = tm * BM, n0 = tn * T;
     const int M = p.m, N = p.n;
+    const int MX = read_m > 0 ? read_m : M, NX = read_n > 0 ? read_n : N;
     const int kbeg = SPLIT ? z * p.k_chunk : 0;
     const int kend = SPLIT ? min(p.k, kbeg + p.k_chunk) : p.k;
     // Whole stages go through the DMA pipeline; a partial last one (k_tail) is staged afterwards.
@@ -238,8 +248,8 @@ __device__ __forceinline__ void half_gemm_dma_tile(const HalfGemmParams& p, int 
     const u16* const pb = static_cast<const u16*>(p.b) + (B_TR ? (size_t)kbeg * p.ldb : (size_t)kbeg);
     Operand<A_TR, BM> opa;
     Operand<B_TR, T> opb;
-    opa.init(pa, p.lda, m0, M, wave, lane);
-    opb.init(pb, p.ldb, n0, N, wave, lane);
+    opa.init(pa, p.lda, m0, MX, wave, lane);
+    opb.init(pb, p.ldb, n0, NX, wave, lane);
     // Last stage index the DMAs clamp to; with no whole stage the pipeline runs on the dummy.
     const int last_st = nst > 0 ? nst - 1 : 0;
     if (nst == 0) {
@@ -378,8 +388,8 @@ __device__ __forceinline__ void half_gemm_dma_tile(const HalfGemmParams& p, int 
     // once every wave has finished reading the buffers, then multiplied like a whole stage.
     if (k_tail > 0) {
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        opa.init(pa, p.lda, m0, M, wave, lane);
-        opb.init(pb, p.ldb, n0, N, wave, lane);
+        opa.init(pa, p.lda, m0, MX, wave, lane);
+        opb.init(pb, p.ldb, n0, NX, wave, lane);
 #pragma unroll
         for (int j = 0; j < NDA; ++j) opa.fill(nst, j, As[0], wave, lane, k_tail);
 #pragma unroll
@@ -388,6 +398,11 @@ __device__ __forceinline__ void half_gemm_dma_tile(const HalfGemmParams& p, int 
         read_half(fa0, fb0, As[0], Bs[0], 0);
         run_half(fa0, fb0, fa1, fb1, As[0], Bs[0], 1, std::false_type{}, 0, 0);
         run_half(fa1, fb1, fa0, fb0, As[0], Bs[0], 0, std::false_type{}, 0, 0);
+    }
+
+    if constexpr (!std::is_same_v<END, StoreTile>) {
+        end(acc, reinterpret_cast<char*>(As), reinterpret_cast<char*>(Bs), m0, n0);
+        return;
     }
 
     // Epilogue through buffer loads and stores relative to the tile's corner.  The byte offset of

@@ -203,9 +203,8 @@ static __device__ __attribute__((aligned(256))) u16 pp_dummy[512];
 struct StoreTile {};
 
 // END: what is made of the finished tile.  StoreTile, or a functor that another operator calls the tile
-// with: end(row, column, v, inside, left) gets 8 adjacent sums v of one row (a row's 256 columns are 32
-// lanes' in order, the two halves of a wave hold adjacent rows, and every lane of the wave calls it);
-// inside: the row lies in the matrix; left: how many columns from `column` on do.
+// with: end(acc, lds, m0, n0) gets the sums as the MFMAs leave them (above), the workgroup's LDS, free
+// once the workgroup has met at a barrier, and the tile's first row and column.
 // read_m, read_n: rows and columns that a's and b's storage holds, where that is more than m and n (a
 // transposed operand is read in whole chunks of 8); 0: m, n.
 template <bool BF16, bool TA, bool TB, class END = StoreTile>
@@ -431,34 +430,7 @@ __device__ __forceinline__ void half_gemm_pp_tile(const HalfGemmParams& p, int b
     }
 
     if constexpr (!std::is_same_v<END, StoreTile>) {
-        // The epilogue's turn through LDS (below), two rows of 512 bytes to an access.
-        const int rows_left = M - m0, er = lane >> 5, ec = 8 * (lane & 31);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            if (128 * i >= rows_left) break;
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-#pragma unroll
-                    for (int v = 0; v < 2; ++v)
-                        *reinterpret_cast<floatx4*>(lds + (64 * wm + 16 * u + j16) * 1024 +
-                                                    16 * ((32 * j + 8 * wn + 4 * v + g) ^ j16)) = acc[i][j][u][v];
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-#pragma unroll
-            for (int t = 0; t < 8; ++t) {
-                const int r = 16 * wave + 2 * t + er, row = 128 * i + r;
-                float out[8];
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const floatx4 f = *reinterpret_cast<const floatx4*>(lds + r * 1024 + 16 * ((ec / 4 + q) ^ (r & 15)));
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) out[4 * q + e] = f[e];
-                }
-                end(m0 + row, n0 + ec, out, row < rows_left, N - n0 - ec);
-            }
-        }
+        end(acc, lds, m0, n0);
         return;
     }
 

@@ -21,7 +21,10 @@ namespace ftrain::train {
 namespace {
 
 constexpr int kThreads     = 256;
-constexpr int kPackThreads = 1024;
+constexpr int kPackThreads = 512;
+constexpr int kFinishThreads = 1024;
+// Most workgroups that pack: two on each of the 256 CUs.
+constexpr int kPackBlocks = 512;
 
 struct PackArgs {
     const void* target;
@@ -32,43 +35,74 @@ struct PackArgs {
     Head* head;
     int32_t* place;  // each token's packed row, -1 if ignored
     RowInfo* rows;
+    const void* x;
+    void* packed;
+    int64_t ld, cols, padded;
+    int64_t per_block;  // tokens
     bool wide, backward, scaled;
 };
 
-// One workgroup: each token's packed row, in order.
-__global__ __launch_bounds__(kPackThreads) void packRows(PackArgs a) {
+// A row of `cols` elements at any address, padded with zeros, by one wave; out: whole 16-byte units.
+template <class T>
+__device__ __forceinline__ void copyRow(const T* from, T* out, int64_t cols, int64_t padded) {
+    constexpr int N     = Pack<T>::kCount;
+    const int lane      = threadIdx.x % kWave;
+    const int64_t whole = cols / N * N;
+#pragma unroll 4
+    for (int64_t i = lane * N; i < whole; i += kWave * N)
+        *reinterpret_cast<Pack<T>*>(out + i) = *reinterpret_cast<const Pack<T>*>(from + i);
+    if (whole + lane < padded) out[whole + lane] = whole + lane < cols ? from[whole + lane] : static_cast<T>(0.f);
+}
+
+// The kept tokens' rows of x, in order and densely.  A workgroup takes `per_block` tokens; it counts the
+// kept ones before them by itself, so that one launch does what a scan and a copy would: 8192 x 4096 bf16
+// 38 us in two launches, 28 in one (134 MB at 4.8 TB/s).
+template <class T>
+__global__ __launch_bounds__(kPackThreads) void packTokens(PackArgs a) {
     constexpr int kWaves = kPackThreads / kWave;
     __shared__ int wave_count[kWaves];
     __shared__ float wave_max[kWaves];
+    __shared__ int place[kPackThreads];
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    auto target = [&](int64_t t) {
-        return a.wide ? static_cast<const int64_t*>(a.target)[t]
-                      : static_cast<int64_t>(static_cast<const int32_t*>(a.target)[t]);
+    auto kept = [&](int64_t t, int64_t& y) {
+        y = a.wide ? static_cast<const int64_t*>(a.target)[t] : static_cast<int64_t>(static_cast<const int32_t*>(a.target)[t]);
+        return y != a.ignore_index;
     };
-    float scale = 1.f;
-    if (a.scaled) {
-        // fp16 holds no small probability: dl is kept times the power of two that brings the largest
-        // |g| into [2^14, 2^15), |dl| <= |g| stays below fp16's largest value, and what is lost is
-        // below 2^-39 of the largest g.
-        float top = 0.f;
+    const int64_t first = blockIdx.x * a.per_block, last = min(first + a.per_block, a.tokens);
+    int64_t y;
+    int count = 0;
+    float top = 0.f;
+#pragma unroll 4
+    for (int64_t t = threadIdx.x; t < first; t += kPackThreads) count += kept(t, y);
+    if (a.scaled)
         for (int64_t t = threadIdx.x; t < a.tokens; t += kPackThreads)
-            if (target(t) != a.ignore_index) top = fmaxf(top, fabsf(a.grad_loss[t]));
-        top = groupMax<kWave>(top);
-        if (lane == 0) wave_max[wave] = top;
-        __syncthreads();
-        for (int w = 0; w < kWaves; ++w) top = fmaxf(top, wave_max[w]);
-        if (top > 0.f && top < INFINITY) {
-            int e;
-            (void)frexpf(top, &e);  // top in [2^(e-1), 2^e)
-            scale = ldexpf(1.f, min(15 - e, 120));
-        }
+            if (kept(t, y)) top = fmaxf(top, fabsf(a.grad_loss[t]));
+    count = groupSum<kWave>(count);
+    top   = groupMax<kWave>(top);
+    if (lane == 0) {
+        wave_count[wave] = count;
+        wave_max[wave]   = top;
     }
+    __syncthreads();
     int before = 0;
-    for (int64_t t0 = 0; t0 < a.tokens; t0 += kPackThreads) {
+    for (int w = 0; w < kWaves; ++w) {
+        before += wave_count[w];
+        top = fmaxf(top, wave_max[w]);
+    }
+    // fp16 holds no small probability: dl is kept times the power of two that brings the largest |g| into
+    // [2^14, 2^15); |dl| <= |g| stays below fp16's largest value, and what is lost is below 2^-39 of the
+    // largest g.
+    float scale = 1.f;
+    if (a.scaled && top > 0.f && top < INFINITY) {
+        int e;
+        (void)frexpf(top, &e);  // top in [2^(e-1), 2^e)
+        scale = ldexpf(1.f, min(15 - e, 120));
+    }
+    for (int64_t t0 = first; t0 < last; t0 += kPackThreads) {
         const int64_t t  = t0 + threadIdx.x;
-        const int64_t y  = t < a.tokens ? target(t) : a.ignore_index;
-        const bool kept  = t < a.tokens && y != a.ignore_index;
-        const unsigned long long mask = __ballot(kept);
+        const bool keeps = t < last && kept(t, y);
+        const unsigned long long mask = __ballot(keeps);
+        __syncthreads();
         if (lane == 0) wave_count[wave] = __popcll(mask);
         __syncthreads();
         int at = before + __popcll(mask & ((1ull << lane) - 1ull));
@@ -76,61 +110,71 @@ __global__ __launch_bounds__(kPackThreads) void packRows(PackArgs a) {
             if (w < wave) at += wave_count[w];
             before += wave_count[w];
         }
-        __syncthreads();
-        if (t < a.tokens) {
-            a.place[t] = kept ? at : -1;
-            if (kept)
+        place[threadIdx.x] = keeps ? at : -1;
+        if (t < last) {
+            a.place[t] = keeps ? at : -1;
+            if (keeps)
                 a.rows[at] = RowInfo{a.backward ? a.lse[t] : 0.f, a.backward ? a.grad_loss[t] * scale : 0.f,
                                      y >= 0 && y < a.classes ? static_cast<int32_t>(y) : -1};
             else if (!a.backward)
                 a.loss[t] = a.lse[t] = 0.f;
         }
+        __syncthreads();
+        for (int64_t i = wave; i < min(last - t0, static_cast<int64_t>(kPackThreads)); i += kWaves)
+            if (place[i] >= 0)
+                copyRow(static_cast<const T*>(a.x) + (t0 + i) * a.ld, static_cast<T*>(a.packed) + place[i] * a.padded, a.cols,
+                        a.padded);
     }
-    if (threadIdx.x == 0) *a.head = Head{before, scale, 1.f / scale};
+    if (threadIdx.x == 0 && blockIdx.x == gridDim.x - 1) *a.head = Head{before, scale, 1.f / scale};
 }
 
-// dst row place[t] (row t with a null place) = src row t, padded with zeros to `padded` columns.
+// A piece of the weight in rows of whole 16-byte units.
 template <class T>
-__global__ __launch_bounds__(kThreads) void copyRows(const T* src, int64_t src_ld, int64_t rows, int64_t cols, T* dst,
-                                                     int64_t dst_ld, int64_t padded, const int32_t* place) {
-    for (int64_t t = blockIdx.x; t < rows; t += gridDim.x) {
-        const int64_t to = place != nullptr ? place[t] : t;
-        if (to < 0) continue;
-        const T* const from = src + t * src_ld;
-        T* const out        = dst + to * dst_ld;
-        constexpr int N     = Pack<T>::kCount;
-        const int64_t whole = cols / N * N;
-        for (int64_t i = threadIdx.x * N; i < whole; i += kThreads * N)
-            *reinterpret_cast<Pack<T>*>(out + i) = *reinterpret_cast<const Pack<T>*>(from + i);
-        for (int64_t i = whole + threadIdx.x; i < padded; i += kThreads) out[i] = i < cols ? from[i] : static_cast<T>(0.f);
-    }
+__global__ __launch_bounds__(kThreads) void packWeight(const T* w, int64_t ld, int64_t rows, int64_t cols, T* out, int64_t padded) {
+    constexpr int kWaves = kThreads / kWave;
+    for (int64_t v = static_cast<int64_t>(blockIdx.x) * kWaves + threadIdx.x / kWave; v < rows; v += static_cast<int64_t>(gridDim.x) * kWaves)
+        copyRow(w + v * ld, out + v * padded, cols, padded);
 }
 
-// loss and lse of every kept token from its tiles' maxima and sums; a wave per token.
-__global__ __launch_bounds__(kThreads) void finishLoss(const float2* part, const float* hit, const RowInfo* rows,
-                                                       const int32_t* place, int64_t tokens, int parts, float* loss,
-                                                       float* lse) {
-    const int lane  = threadIdx.x % kWave;
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * (kThreads / kWave) + threadIdx.x / kWave;
-    if (t >= tokens) return;
-    const int row = place[t];
-    if (row < 0) return;
-    const float2* const mine = part + static_cast<int64_t>(row) * parts;
-    float top = -INFINITY;
-    for (int i = lane; i < parts; i += kWave) top = fmaxf(top, mine[i].x);
-    top = groupMax<kWave>(top);
-    float sum = 0.f;
-    for (int i = lane; i < parts; i += kWave) {
-        const float2 v = mine[i];
-        // A tile of nothing but minus infinity has no sum.
-        sum += v.x == -INFINITY && top > -INFINITY ? 0.f : v.y * expf(v.x - top);
+// loss and lse of every kept token from its parts' maxima and sums: lanes take adjacent tokens, the
+// workgroup's waves every kWaves-th part, eight loads in flight.
+__global__ __launch_bounds__(kFinishThreads) void finishLoss(const float2* part, const float* hit, const RowInfo* rows,
+                                                             const int32_t* place, int64_t tokens, int parts, float* loss,
+                                                             float* lse) {
+    constexpr int kWaves = kFinishThreads / kWave, kBatch = 8;
+    __shared__ float2 met[kWaves][kWave];
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * kWave + lane;
+    const int row   = t < tokens ? place[t] : -1;
+    float top = -INFINITY, sum = 0.f;
+    // (top, sum) and v's joined; minus infinity has no sum.
+    auto join = [&](auto& v) {
+        float high = top;
+        for (const float2& x : v) high = fmaxf(high, x.x);
+        const float base = high == -INFINITY ? 0.f : high;
+        sum *= expf(top - base);
+        for (const float2& x : v) sum += x.y * expf(x.x - base);
+        top = high;
+    };
+    if (row >= 0) {
+        for (int i = wave; i < parts; i += kWaves * kBatch) {
+            float2 v[kBatch];
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b)
+                v[b] = i + b * kWaves < parts ? part[(i + b * kWaves) * tokens + row] : make_float2(-INFINITY, 0.f);
+            join(v);
+        }
     }
-    sum = groupSum<kWave>(sum);
-    if (lane == 0) {
-        const float l = top + logf(sum);
-        lse[t]        = l;
-        loss[t]       = rows[row].target < 0 ? NAN : l - hit[row];
-    }
+    met[wave][lane] = make_float2(top, sum);
+    __syncthreads();
+    if (wave != 0 || row < 0) return;
+    float2 v[kWaves - 1];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) v[w - 1] = met[w][lane];
+    join(v);
+    const float l = top + logf(sum);
+    lse[t]        = l;
+    loss[t]       = rows[row].target < 0 ? NAN : l - hit[row];
 }
 
 // grad_hidden row t: the packed row's sums, rounded once; zeros for an ignored token.
@@ -164,8 +208,47 @@ uint64_t roundUp(uint64_t a, uint64_t b) { return ceilDiv(a, b) * b; }
 
 // Bytes of a piece of dl: the last-level cache's 256 MiB, which it is read from twice.
 constexpr uint64_t kPieceBytes = 256ull << 20;
-// Workgroups that fill the device's 256 CUs.
-constexpr uint64_t kFill = 256;
+constexpr uint64_t kCus = 256;
+
+// How a product runs: tile rows and columns, and slices of k that keep sums of their own.
+struct Tiling {
+    int size;
+    int slices;
+};
+
+// Modelled time of an m x n x k product, us: rounds of the 256 CUs, each of its stages and a start and
+// end.  Measured per stage: 16-bit (64 k) 256x256 1.25 (0.75 with at most 128 rows), 128x128 0.5; fp32
+// (32 k) 128x128 1.75, 64x64 0.5.  A large tile reads less for each product, a small one fills the CUs
+// where there are few:
+//   bf16, us, 256x256 / 128x128: loss of 128 x 1024 x 8192 27.8 / 24.0, 500 x 1024 x 5003 40.5 / 23.2,
+//     64 x 4096 x 128000 201 / 234; gradients of 500 x 1024 x 5003 77.6 / 60.2, 2048 x 4096 x 32003
+//     1198 / 1392;
+//   fp32, us, 128x128 / 64x64: loss of 300 x 8192 x 3000 470 / 166, 1000 x 1000 x 1000 80 / 36.
+double tileMicros(bool fp32, int size, int64_t m, int64_t n, int64_t k, int slices) {
+    const double stage = fp32 ? (size == 128 ? 1.75 : 0.5) : size == 256 ? (m <= 128 ? 0.75 : 1.25) : 0.5;
+    const double ends  = fp32 ? 5.0 : size == 256 ? 9.0 : 6.0;
+    const uint64_t rounds = ceilDiv(ceilDiv(m, size) * ceilDiv(n, size) * slices, kCus);
+    return static_cast<double>(rounds) * (static_cast<double>(ceilDiv(k, slices)) / (fp32 ? 32 : 64) * stage + ends);
+}
+
+// sliced: k may be cut until the tiles fill the device (two fp32 workgroups run on a CU), in slices of
+// at least 512.
+Tiling tilingOf(FTrainNumericType type, int64_t m, int64_t n, int64_t k, bool sliced) {
+    const bool fp32 = type == FTRAIN_NUMERIC_TYPE_FP32;
+    Tiling best{};
+    double least = 0.0;
+    for (const int size : {fp32 ? 128 : 256, fp32 ? 64 : 128}) {
+        const uint64_t tiles = std::max<uint64_t>(1, ceilDiv(m, size) * ceilDiv(n, size));
+        int slices           = 1;
+        if (sliced) slices = static_cast<int>(std::max<uint64_t>(1, std::min<uint64_t>((fp32 ? 2 : 1) * kCus / tiles, k / 512)));
+        const double micros = tileMicros(fp32, size, m, n, k, slices);
+        if (best.size == 0 || micros < least) {
+            best  = {size, slices};
+            least = micros;
+        }
+    }
+    return best;
+}
 
 // The workspace, laid out for one call.
 struct Layout {
@@ -174,7 +257,7 @@ struct Layout {
     int64_t padded;  // columns of a packed row of x (and w)
     int64_t piece;   // classes of one piece
     int64_t parts;
-    int slices;      // of a piece's classes, each with sums of its own for dx
+    Tiling logits, for_hidden, for_weight;
     int64_t slice;   // elements of one slice's sums
     bool pack_w;     // the weight's rows are not whole 16-byte units: each piece is copied first
 
@@ -185,12 +268,15 @@ struct Layout {
         pack_w = hidden % unit != 0 || p.weight.ld % unit != 0 || reinterpret_cast<uintptr_t>(p.weight.data) % 16 != 0;
         const uint64_t row = backward ? tokens * size : pack_w ? padded * size : 1;
         piece = std::min(std::max<uint64_t>(kPieceBytes / std::max<uint64_t>(row, 1) / 256 * 256, 2048), roundUp(classes, 256));
-        parts = ceilDiv(classes, headPartClasses(p.type));
-        const uint64_t tile  = p.type == FTRAIN_NUMERIC_TYPE_FP32 ? 128 : 256;
-        const uint64_t tiles = std::max<uint64_t>(1, ceilDiv(tokens, tile) * ceilDiv(hidden, tile));
-        slices               = static_cast<int>(std::max<uint64_t>(1, std::min(kFill / tiles, static_cast<uint64_t>(piece) / 512)));
-        slice                = tokens * padded;
-        auto take            = [&](uint64_t n) {
+        const int64_t n = backward || pack_w ? std::min<int64_t>(piece, classes) : classes;
+        logits          = tilingOf(p.type, tokens, n, padded, false);
+        // Classes of one part: of a 16-bit tile's columns, or of the 64 that an fp32 wave holds.
+        parts      = ceilDiv(classes, p.type == FTRAIN_NUMERIC_TYPE_FP32 ? 64 : logits.size);
+        for_hidden = tilingOf(p.type, tokens, hidden, n, true);
+        // The rows of the weight's gradient are the classes: always many, so fp32 has the large tile only.
+        for_weight = p.type == FTRAIN_NUMERIC_TYPE_FP32 ? Tiling{128, 1} : tilingOf(p.type, n, hidden, tokens, false);
+        slice     = tokens * padded;
+        auto take = [&](uint64_t n) {
             const uint64_t at = bytes;
             bytes += roundUp(n, 256);
             return at;
@@ -203,7 +289,7 @@ struct Layout {
         part  = backward ? 0 : take(tokens * parts * sizeof(float2));
         hit   = backward ? 0 : take(tokens * 4);
         dl    = backward ? take(tokens * piece * size) : 0;
-        dx    = backward ? take(slices * slice * 4) : 0;
+        dx    = backward ? take(for_hidden.slices * slice * 4) : 0;
     }
 };
 
@@ -218,14 +304,27 @@ template <class T>
 Buffers packInputs(const CrossEntropy& p, const Layout& l, char* base, bool backward, hipStream_t stream) {
     Buffers b{reinterpret_cast<Head*>(base + l.head), reinterpret_cast<int32_t*>(base + l.place),
               reinterpret_cast<RowInfo*>(base + l.rows), base};
-    PackArgs a{p.target, p.ignore_index, p.hidden.rows, p.weight.rows, p.loss, p.lse, p.grad_loss, b.head,
-               b.place,  b.rows,         p.target_wide, backward,      backward && p.type == FTRAIN_NUMERIC_TYPE_FP16};
-    launch(&packRows, "cross entropy pack", dim3(1), dim3(kPackThreads), stream, a);
-    if (p.hidden.rows > 0)
-        launch(&copyRows<T>, "cross entropy copy", dim3(static_cast<uint32_t>(std::min<int64_t>(p.hidden.rows, 65536))),
-           dim3(kThreads), stream, static_cast<const T*>(p.hidden.data), p.hidden.ld, p.hidden.rows, p.hidden.cols,
-           reinterpret_cast<T*>(base + l.x), l.padded, l.padded, static_cast<const int32_t*>(b.place));
+    PackArgs a{};
+    a.target = p.target, a.ignore_index = p.ignore_index, a.wide = p.target_wide;
+    a.tokens = p.hidden.rows, a.classes = p.weight.rows;
+    a.loss = p.loss, a.lse = p.lse, a.grad_loss = p.grad_loss;
+    a.head = b.head, a.place = b.place, a.rows = b.rows;
+    a.x = p.hidden.data, a.ld = p.hidden.ld, a.cols = p.hidden.cols;
+    a.packed = base + l.x, a.padded = l.padded;
+    a.backward = backward, a.scaled = backward && p.type == FTRAIN_NUMERIC_TYPE_FP16;
+    a.per_block        = std::max<int64_t>(1, ceilDiv(a.tokens, kPackBlocks));
+    const int64_t grid = std::max<int64_t>(1, ceilDiv(a.tokens, a.per_block));
+    launch(&packTokens<T>, "cross entropy pack", dim3(static_cast<uint32_t>(grid)), dim3(kPackThreads), stream, a);
     return b;
+}
+
+void launchHeadTile(FTrainNumericType type, HeadTile what, int size, const HeadTileArgs& args, int slices, hipStream_t stream) {
+    if (type == FTRAIN_NUMERIC_TYPE_FP32)
+        launchHeadTileFp32(what, size, args, slices, stream);
+    else if (type == FTRAIN_NUMERIC_TYPE_BF16)
+        launchHeadTileBf16(what, size, args, slices, stream);
+    else
+        launchHeadTileFp16(what, size, args, slices, stream);
 }
 
 // The classes from `first` on, `n` of them, in rows of whole 16-byte units.
@@ -236,8 +335,8 @@ const T* weightPiece(const CrossEntropy& p, const Layout& l, char* base, int64_t
     ld                  = p.weight.ld;
     if (!l.pack_w) return from;
     T* const to = reinterpret_cast<T*>(base + l.w);
-    launch(&copyRows<T>, "cross entropy weight copy", dim3(static_cast<uint32_t>(std::min<int64_t>(n, 65536))), dim3(kThreads),
-           stream, from, p.weight.ld, n, p.weight.cols, to, l.padded, l.padded, static_cast<const int32_t*>(nullptr));
+    launch(&packWeight<T>, "cross entropy weight pack", dim3(static_cast<uint32_t>(std::min<int64_t>(ceilDiv(n, 4), 4096))),
+           dim3(kThreads), stream, from, p.weight.ld, n, p.weight.cols, to, l.padded);
     ld = l.padded;
     return to;
 }
@@ -251,15 +350,15 @@ void forward(const CrossEntropy& p, char* base, hipStream_t stream) {
     t.m = p.hidden.rows, t.k = l.padded;
     t.head = b.head, t.rows = b.rows;
     t.part = reinterpret_cast<float2*>(base + l.part), t.hit = reinterpret_cast<float*>(base + l.hit);
-    t.parts              = l.parts;
+    t.tokens              = p.hidden.rows;
     const int64_t classes = p.weight.rows, piece = l.pack_w ? l.piece : classes;
     for (int64_t v = 0; v < classes; v += piece) {
         t.n = std::min(piece, classes - v), t.first_class = v;
         t.b = weightPiece<T>(p, l, base, v, t.n, t.ldb, stream);
-        launchHeadTile(p.type, HeadTile::kLogSum, t, 1, stream);
+        launchHeadTile(p.type, HeadTile::kLogSum, l.logits.size, t, 1, stream);
     }
-    launch(&finishLoss, "cross entropy loss", dim3(static_cast<uint32_t>(ceilDiv(p.hidden.rows, kThreads / kWave))),
-           dim3(kThreads), stream, static_cast<const float2*>(t.part), static_cast<const float*>(t.hit),
+    launch(&finishLoss, "cross entropy loss", dim3(static_cast<uint32_t>(ceilDiv(p.hidden.rows, kWave))),
+           dim3(kFinishThreads), stream, static_cast<const float2*>(t.part), static_cast<const float*>(t.hit),
            static_cast<const RowInfo*>(b.rows), static_cast<const int32_t*>(b.place), p.hidden.rows,
            static_cast<int>(l.parts), p.loss, p.lse);
 }
@@ -281,45 +380,34 @@ void backward(const CrossEntropy& p, char* base, hipStream_t stream) {
             t.b = w, t.ldb = ldw;
             t.d = base + l.dl, t.ldd = l.piece;
             t.m = tokens, t.n = n, t.k = l.padded;
-            launchHeadTile(p.type, HeadTile::kGradLogits, t, 1, stream);
+            launchHeadTile(p.type, HeadTile::kGradLogits, l.logits.size, t, 1, stream);
             t.a = base + l.dl, t.lda = l.piece;
             t.d = base + l.dx, t.ldd = l.padded;
             t.n = l.padded, t.k = n;
             // Whole stages of the tile to a slice; a last piece's slices may be fewer, its sums then
             // leave the others as they are.
-            t.k_chunk        = roundUp(ceilDiv(n, l.slices), 64);
+            t.k_chunk        = roundUp(ceilDiv(n, l.for_hidden.slices), 64);
             t.slice          = l.slice;
             t.add            = v > 0;
-            const int slices = t.add ? static_cast<int>(ceilDiv(n, t.k_chunk)) : l.slices;
-            launchHeadTile(p.type, HeadTile::kGradHidden, t, slices, stream);
+            const int slices = t.add ? static_cast<int>(ceilDiv(n, t.k_chunk)) : l.for_hidden.slices;
+            launchHeadTile(p.type, HeadTile::kGradHidden, l.for_hidden.size, t, slices, stream);
         }
         t.a = base + l.dl, t.lda = l.piece;
         t.b = base + l.x, t.ldb = l.padded;
         t.d = static_cast<T*>(p.grad_weight.data) + v * p.grad_weight.ld, t.ldd = p.grad_weight.ld;
         t.m = n, t.n = hidden, t.k = tokens;
         t.read_m = roundUp(n, unit), t.read_n = l.padded;
-        launchHeadTile(p.type, HeadTile::kGradWeight, t, 1, stream);
+        launchHeadTile(p.type, HeadTile::kGradWeight, l.for_weight.size, t, 1, stream);
     }
     if (tokens > 0)
         launch(&finishHidden<T>, "cross entropy hidden gradient's rows",
                dim3(static_cast<uint32_t>(std::min<int64_t>(tokens, 65536))), dim3(kThreads), stream,
                reinterpret_cast<const float*>(base + l.dx), l.padded, static_cast<const int32_t*>(b.place),
                static_cast<const Head*>(b.head), static_cast<T*>(p.grad_hidden.data), p.grad_hidden.ld, tokens, hidden,
-               l.slices, l.slice);
+               l.for_hidden.slices, l.slice);
 }
 
 }  // namespace
-
-int headPartClasses(FTrainNumericType type) { return type == FTRAIN_NUMERIC_TYPE_FP32 ? 64 : 256; }
-
-void launchHeadTile(FTrainNumericType type, HeadTile what, const HeadTileArgs& args, int slices, hipStream_t stream) {
-    if (type == FTRAIN_NUMERIC_TYPE_FP32)
-        launchHeadTileFp32(what, args, slices, stream);
-    else if (type == FTRAIN_NUMERIC_TYPE_BF16)
-        launchHeadTileBf16(what, args, slices, stream);
-    else
-        launchHeadTileFp16(what, args, slices, stream);
-}
 
 uint64_t crossEntropyWorkspace(const CrossEntropy& p, bool backward) { return Layout(p, backward).bytes; }
 

@@ -41,10 +41,11 @@ struct HeadTileArgs {
     const Head* head;
     const RowInfo* rows;
     int32_t first_class;
-    // kLogSum: of each row, `parts` pairs of maximum and sum, and the logit of its target.
+    // kLogSum: a pair of maximum and sum of each part of the classes and, within it, of each of `tokens`
+    // rows; the logit of each row's target.
     float2* part;
     float* hit;
-    int32_t parts;
+    int64_t tokens;
     // kGradHidden: the classes of one of gridDim.z slices, elements from one slice's sums to the next's,
     // and whether the sums of earlier classes are added to.
     int32_t k_chunk;
@@ -52,13 +53,10 @@ struct HeadTileArgs {
     bool add;
 };
 
-// Classes whose maximum and sum one tile leaves in one pair.
-int headPartClasses(FTrainNumericType type);
-// Launches the product; m counts every token, the kernels take the packed ones only.
-void launchHeadTile(FTrainNumericType type, HeadTile what, const HeadTileArgs& args, int slices, hipStream_t stream);
-
-void launchHeadTileFp32(HeadTile what, const HeadTileArgs& args, int slices, hipStream_t stream);
-void launchHeadTileBf16(HeadTile what, const HeadTileArgs& args, int slices, hipStream_t stream);
-void launchHeadTileFp16(HeadTile what, const HeadTileArgs& args, int slices, hipStream_t stream);
+// Launches the product on tiles of `size` rows and columns; m counts every token, the kernels take the
+// packed ones only.
+void launchHeadTileFp32(HeadTile what, int size, const HeadTileArgs& args, int slices, hipStream_t stream);
+void launchHeadTileBf16(HeadTile what, int size, const HeadTileArgs& args, int slices, hipStream_t stream);
+void launchHeadTileFp16(HeadTile what, int size, const HeadTileArgs& args, int slices, hipStream_t stream);
 
 }  // namespace ftrain::train

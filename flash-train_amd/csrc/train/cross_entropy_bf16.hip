@@ -3,8 +3,8 @@
 
 namespace ftrain::train {
 
-void launchHeadTileBf16(HeadTile what, const HeadTileArgs& args, int slices, hipStream_t stream) {
-    launchHeadTileHalf<true>(what, args, slices, stream);
+void launchHeadTileBf16(HeadTile what, int size, const HeadTileArgs& args, int slices, hipStream_t stream) {
+    launchHeadTileHalf<true>(what, size, args, slices, stream);
 }
 
 }  // namespace ftrain::train

@@ -3,22 +3,13 @@
 
 namespace ftrain::train {
 
-void launchHeadTileFp32(HeadTile what, const HeadTileArgs& args, int slices, hipStream_t stream) {
-    const dim3 grid = headGrid(args, 128, slices);
-    switch (what) {
-        case HeadTile::kLogSum:
-            launch(&headTileFp32<HeadTile::kLogSum>, "cross entropy logits", grid, dim3(256), stream, args);
-            break;
-        case HeadTile::kGradLogits:
-            launch(&headTileFp32<HeadTile::kGradLogits>, "cross entropy logits' gradient", grid, dim3(256), stream, args);
-            break;
-        case HeadTile::kGradHidden:
-            launch(&headTileFp32<HeadTile::kGradHidden>, "cross entropy hidden gradient", grid, dim3(256), stream, args);
-            break;
-        case HeadTile::kGradWeight:
-            launch(&headTileFp32<HeadTile::kGradWeight>, "cross entropy weight gradient", grid, dim3(256), stream, args);
-            break;
-    }
+void launchHeadTileFp32(HeadTile what, int size, const HeadTileArgs& args, int slices, hipStream_t stream) {
+    constexpr void (*large[4])(HeadTileArgs) = {&headTileFp32<HeadTile::kLogSum, 128>, &headTileFp32<HeadTile::kGradLogits, 128>,
+                                                &headTileFp32<HeadTile::kGradHidden, 128>, &headTileFp32<HeadTile::kGradWeight, 128>};
+    constexpr void (*small[3])(HeadTileArgs) = {&headTileFp32<HeadTile::kLogSum, 64>, &headTileFp32<HeadTile::kGradLogits, 64>,
+                                                &headTileFp32<HeadTile::kGradHidden, 64>};
+    const int i = static_cast<int>(what);
+    launchHead(size == 128 ? large[i] : small[i], kHeadNames[i], args, size, 256, slices, stream);
 }
 
 }  // namespace ftrain::train

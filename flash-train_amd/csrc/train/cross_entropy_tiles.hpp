@@ -1,8 +1,10 @@
-// The cross entropy's products on the GEMM's tiles (gemm/pingpong_tile.hpp for 16-bit types,
-// gemm/dma32_tile.hpp for fp32), with the ends below in place of d = alpha acc + beta c.
+// The cross entropy's products on the GEMM's tiles, with the ends below in place of d = alpha acc + beta c:
+// 16-bit types on 256x256 (gemm/pingpong_tile.hpp) and 128x128 (gemm/dma_tile.hpp), fp32 on 128x128 and
+// 64x64 (gemm/dma32_tile.hpp).
 #pragma once
 
 #include "../gemm/dma32_tile.hpp"
+#include "../gemm/dma_tile.hpp"
 #include "../gemm/pingpong_tile.hpp"
 #include "cross_entropy.hpp"
 #include "device.hpp"
@@ -14,56 +16,333 @@ namespace ftrain::train {
 // logits' own sums are.
 __device__ __forceinline__ float expFast(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
-// A row's largest logit and sum of exponentials over the N * LANES classes that its lanes hold.
-template <int N, int LANES>
-struct LogSumEnd {
+// ---- 16-bit operands: the 256x256 tile of gemm/pingpong_tile.hpp.
+//
+// A lane holds, of row 128 i + 64 wm + 16 u + j16 of the tile, columns 128 j + 32 wn + 16 v + 4 g + r
+// (i, j, v < 2, u, r < 4): acc[i][j][u][v][r].
+typedef gemm::ppdev::floatx4 TileSums[2][2][4][2];
+
+struct Place {
+    int lane, j16, g, wm, wn, wave;
+    __device__ __forceinline__ Place()
+        : lane(threadIdx.x & 63), j16(lane & 15), g(lane >> 4),
+          wm(__builtin_amdgcn_readfirstlane(threadIdx.x >> 8)),
+          wn(__builtin_amdgcn_readfirstlane((threadIdx.x >> 6) & 3)),
+          wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) {}
+    __device__ __forceinline__ int row(int i, int u) const { return 128 * i + 64 * wm + 16 * u + j16; }
+    __device__ __forceinline__ int col(int j, int v) const { return 128 * j + 32 * wn + 16 * v + 4 * g; }
+};
+
+// Each row's largest logit and sum of exponentials over the tile's classes.  A lane reduces its 16
+// logits of a row by itself, four lanes meet by shuffles, four waves in LDS.  Against a turn of the tile
+// through LDS, after which 32 lanes hold a row (ten shuffles for every two rows of a wave): 8192 x 4096 x
+// 65536 bf16 3156 -> 2838 us.
+struct LogSumEnd16 {
     const RowInfo* rows;
     float2* part;
     float* hit;
-    int parts, first_class;
+    int64_t tokens;
+    int M, N, first_class;
 
-    __device__ __forceinline__ void operator()(int row, int col, float (&v)[N], bool inside, int left) const {
-        float top = -INFINITY;
+    __device__ __forceinline__ void operator()(TileSums& acc, char* lds, int m0, int n0) const {
+        const Place at;
+        const int rows_left = M - m0, cols_left = N - n0;
+        if (cols_left < 256) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            if (e >= left) v[e] = -INFINITY;
-            top = fmaxf(top, v[e]);
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int v = 0; v < 2; ++v)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (at.col(j, v) + r >= cols_left) {
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                                for (int u = 0; u < 4; ++u) acc[i][j][u][v][r] = -INFINITY;
+                        }
         }
-        top       = groupMax<LANES>(top);
-        float sum = 0.f;
+        float2* const met = reinterpret_cast<float2*>(lds);  // [4][256]
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
-        for (int e = 0; e < N; ++e) sum += e < left ? expFast(v[e] - top) : 0.f;
-        sum = groupSum<LANES>(sum);
-        if (!inside) return;
-        const int at = rows[row].target - first_class - col;
+        for (int i = 0; i < 2; ++i) {
+            if (128 * i >= rows_left) break;
+            int target[4];
 #pragma unroll
-        for (int e = 0; e < N; ++e)
-            if (e == at && e < left) hit[row] = v[e];
-        // (A group may lie past the classes.)
-        if (threadIdx.x % LANES == 0 && left > 0)
-            part[static_cast<int64_t>(row) * parts + (first_class + col) / (N * LANES)] = make_float2(top, sum);
+            for (int u = 0; u < 4; ++u) {
+                const int row = at.row(i, u);
+                target[u]     = row < rows_left ? rows[m0 + row].target - first_class - n0 : -1;
+            }
+            float top[4], sum[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                top[u] = acc[i][0][u][0][0];
+#pragma unroll
+                for (int q = 1; q < 16; ++q) top[u] = fmaxf(top[u], acc[i][q >> 3][u][(q >> 2) & 1][q & 3]);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) top[u] = fmaxf(top[u], __shfl_xor(top[u], 16, kWave));
+#pragma unroll
+            for (int u = 0; u < 4; ++u) top[u] = fmaxf(top[u], __shfl_xor(top[u], 32, kWave));
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                // Nothing but minus infinity: the exponentials of the differences would be NaN.
+                const float base = top[u] == -INFINITY ? 0.f : top[u];
+                sum[u]           = 0.f;
+#pragma unroll
+                for (int q = 0; q < 16; ++q) sum[u] += expFast(acc[i][q >> 3][u][(q >> 2) & 1][q & 3] - base);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) sum[u] += __shfl_xor(sum[u], 16, kWave);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) sum[u] += __shfl_xor(sum[u], 32, kWave);
+            if (at.g == 0) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) met[256 * at.wn + at.row(i, u)] = make_float2(top[u], sum[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int t   = target[u];
+                const bool my = t >= 0 && t < min(256, cols_left) && ((t >> 5) & 3) == at.wn && ((t >> 2) & 3) == at.g;
+                if (__any(my)) {
+                    float x = 0.f;
+#pragma unroll
+                    for (int q = 0; q < 16; ++q)
+                        if ((t >> 7) == (q >> 3) && ((t >> 4) & 1) == ((q >> 2) & 1) && (t & 3) == (q & 3))
+                            x = acc[i][q >> 3][u][(q >> 2) & 1][q & 3];
+                    if (my) hit[m0 + at.row(i, u)] = x;
+                }
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        const int row = threadIdx.x;
+        if (row < 256 && row < rows_left) {
+            float2 s[4];
+            float top = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                s[w] = met[256 * w + row];
+                top  = fmaxf(top, s[w].x);
+            }
+            const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) sum += s[w].y * expFast(s[w].x - base);
+            part[static_cast<int64_t>((first_class + n0) >> 8) * tokens + m0 + row] = make_float2(top, sum);
+        }
     }
 };
 
 // dl in the operands' type: g (exp(l - lse) - [the target]), zeros in the padding past the classes.
-template <class T, int N>
-struct GradLogitsEnd {
+// Formed where the MFMAs leave it, then turned through LDS (512 bytes a row, 16-byte chunk c of row r at
+// slot c ^ (r & 15): no bank conflicts) so that a store covers two rows of 512 bytes.
+template <bool BF16>
+struct GradLogitsEnd16 {
+    using T = std::conditional_t<BF16, bf16, fp16>;
     const RowInfo* rows;
     T* d;
     int64_t ldd;
+    int M, N, padded, first_class;
+
+    __device__ __forceinline__ void operator()(TileSums& acc, char* lds, int m0, int n0) const {
+        typedef gemm::ppdev::u32x4 u32x4;
+        typedef gemm::ppdev::u32x2 u32x2;
+        const Place at;
+        const int rows_left = M - m0, cols_left = N - n0;
+        RowInfo info[2][4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) info[i][u] = rows[m0 + min(at.row(i, u), rows_left - 1)];
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (128 * i >= rows_left) break;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const RowInfo r = info[i][u];
+                const int y     = r.target - first_class - n0;
+                const float g   = r.target < 0 ? NAN : r.grad;
+                char* const to  = lds + at.row(i, u) * 512;
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int v = 0; v < 2; ++v) {
+                        const int c = at.col(j, v);
+                        float x[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            x[e] = (expFast(acc[i][j][u][v][e] - r.lse) - (c + e == y ? 1.f : 0.f)) * g;
+                            if (c + e >= cols_left) x[e] = 0.f;
+                        }
+                        *reinterpret_cast<u32x2*>(to + 16 * ((c >> 3) ^ at.j16) + 8 * (at.g & 1)) =
+                            u32x2{gemm::ppdev::pack2<BF16>(x[0], x[1]), gemm::ppdev::pack2<BF16>(x[2], x[3])};
+                    }
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        const int er = at.lane >> 5, ec = 8 * (at.lane & 31);
+#pragma unroll
+        for (int t = 0; t < 16; ++t) {
+            const int row = 32 * at.wave + 2 * t + er;
+            if (row < rows_left && n0 + ec < padded)
+                *reinterpret_cast<u32x4*>(d + (m0 + row) * ldd + n0 + ec) =
+                    *reinterpret_cast<const u32x4*>(lds + row * 512 + 16 * ((ec >> 3) ^ (row & 15)));
+        }
+    }
+};
+
+// ---- 16-bit operands: the 128x128 tile of gemm/dma_tile.hpp.
+//
+// Lane (li = lane % 32, h = lane / 32) of wave w holds rows 64 (w / 2) + 32 bi + 8 (r / 4) + 4 h + r % 4,
+// column 64 (w % 2) + 32 bj + li: acc[bi][bj][r].  Both ends turn the tile through LDS (512 bytes a row;
+// the row's halves change places where bit 2 of the row is set, so the two h write to different banks),
+// after which 16 lanes hold 8 adjacent columns each of a row and a wave four rows.
+typedef gemm::ddev::floatx16 TileSums128[2][2];
+
+// f(row, column, v[8]) for the 8 steps of every wave, rows and columns within the tile.
+template <class F>
+__device__ __forceinline__ void turned128(TileSums128& acc, char* a, char* b, F&& f) {
+    typedef gemm::ppdev::floatx4 floatx4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // Rows 0 .. 63, which waves 0 and 1 hold and read again, in a's LDS, the others in b's.
+    char* const lds = wave < 2 ? a : b - 64 * 512;
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+    for (int bi = 0; bi < 2; ++bi)
+#pragma unroll
+        for (int bj = 0; bj < 2; ++bj)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int row = 64 * (wave >> 1) + 32 * bi + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
+                const int col = 64 * (wave & 1) + 32 * bj + (lane & 31);
+                *reinterpret_cast<float*>(lds + row * 512 + 4 * (col ^ (8 * (row & 4)))) = acc[bi][bj][r];
+            }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+        const int row = 32 * wave + 4 * t + (lane >> 4), col = 8 * (lane & 15);
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const floatx4 x = *reinterpret_cast<const floatx4*>(lds + row * 512 + 4 * ((col + 4 * q) ^ (8 * (row & 4))));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[4 * q + e] = x[e];
+        }
+        f(t, row, col, v);
+    }
+}
+
+struct LogSumEnd128 {
+    const RowInfo* rows;
+    float2* part;
+    float* hit;
+    int64_t tokens;
+    int M, N, first_class;
+
+    __device__ __forceinline__ void operator()(TileSums128& acc, char* a, char* b, int m0, int n0) const {
+        const int rows_left = M - m0, cols_left = N - n0, own = 32 * (threadIdx.x >> 6) + ((threadIdx.x & 63) >> 4);
+        int target[8];
+#pragma unroll
+        for (int t = 0; t < 8; ++t) target[t] = rows[m0 + min(own + 4 * t, rows_left - 1)].target - first_class - n0;
+        turned128(acc, a, b, [&](int t, int row, int col, float (&v)[8]) {
+            float top = -INFINITY, sum = 0.f, x = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (col + e >= cols_left) v[e] = -INFINITY;
+                if (col + e == target[t]) x = v[e];
+                top = fmaxf(top, v[e]);
+            }
+            top              = groupMax<16>(top);
+            const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum += expFast(v[e] - base);
+            sum = groupSum<16>(sum);
+            if (row >= rows_left) return;
+            if (target[t] >= col && target[t] < min(col + 8, cols_left)) hit[m0 + row] = x;
+            if (col == 0) part[static_cast<int64_t>((first_class + n0) >> 7) * tokens + m0 + row] = make_float2(top, sum);
+        });
+    }
+};
+
+template <bool BF16>
+struct GradLogitsEnd128 {
+    using T = std::conditional_t<BF16, bf16, fp16>;
+    const RowInfo* rows;
+    T* d;
+    int64_t ldd;
+    int M, N, padded, first_class;
+
+    __device__ __forceinline__ void operator()(TileSums128& acc, char* a, char* b, int m0, int n0) const {
+        using gemm::ppdev::pack2;
+        const int rows_left = M - m0, cols_left = N - n0, own = 32 * (threadIdx.x >> 6) + ((threadIdx.x & 63) >> 4);
+        RowInfo info[8];
+#pragma unroll
+        for (int t = 0; t < 8; ++t) info[t] = rows[m0 + min(own + 4 * t, rows_left - 1)];
+        turned128(acc, a, b, [&](int t, int row, int col, float (&v)[8]) {
+            const RowInfo r = info[t];
+            const int y     = r.target - first_class - n0;
+            const float g   = r.target < 0 ? NAN : r.grad;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[e] = (expFast(v[e] - r.lse) - (col + e == y ? 1.f : 0.f)) * g;
+                if (col + e >= cols_left) v[e] = 0.f;
+            }
+            if (row < rows_left && n0 + col < padded)
+                *reinterpret_cast<gemm::ppdev::u32x4*>(d + (m0 + row) * ldd + n0 + col) = gemm::ppdev::u32x4{
+                    pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]), pack2<BF16>(v[4], v[5]), pack2<BF16>(v[6], v[7])};
+        });
+    }
+};
+
+// ---- fp32: the tiles of gemm/dma32_tile.hpp, four adjacent sums of a row at a time.
+
+// A row's largest logit and sum of exponentials over the 64 classes that 16 lanes hold.
+struct LogSumEnd32 {
+    const RowInfo* rows;
+    float2* part;
+    float* hit;
+    int64_t tokens;
+    int first_class;
+
+    __device__ __forceinline__ void operator()(int row, int col, float (&v)[4], bool inside, int left) const {
+        float top = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (e >= left) v[e] = -INFINITY;
+            top = fmaxf(top, v[e]);
+        }
+        top              = groupMax<16>(top);
+        const float base = top == -INFINITY ? 0.f : top;
+        float sum        = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum += expFast(v[e] - base);
+        sum = groupSum<16>(sum);
+        if (!inside) return;
+        const int at = rows[row].target - first_class - col;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e == at && e < left) hit[row] = v[e];
+        // (The lanes' classes may all lie past the last.)
+        if (threadIdx.x % 16 == 0 && left > 0)
+            part[static_cast<int64_t>((first_class + col) >> 6) * tokens + row] = make_float2(top, sum);
+    }
+};
+
+struct GradLogitsEnd32 {
+    const RowInfo* rows;
+    float* d;
+    int64_t ldd;
     int padded, first_class;
 
-    __device__ __forceinline__ void operator()(int row, int col, float (&v)[N], bool inside, int left) const {
+    __device__ __forceinline__ void operator()(int row, int col, float (&v)[4], bool inside, int left) const {
         if (!inside || col >= padded) return;
         const RowInfo r = rows[row];
         const int at    = r.target - first_class - col;
         const float g   = r.target < 0 ? NAN : r.grad;
-        typedef T vec __attribute__((ext_vector_type(N)));
-        vec out;
+        float4 out;
+        float* const o = &out.x;
 #pragma unroll
-        for (int e = 0; e < N; ++e)
-            out[e] = static_cast<T>(e < left ? (expFast(v[e] - r.lse) - (e == at ? 1.f : 0.f)) * g : 0.f);
-        *reinterpret_cast<vec*>(d + row * ldd + col) = out;
+        for (int e = 0; e < 4; ++e) o[e] = e < left ? (expFast(v[e] - r.lse) - (e == at ? 1.f : 0.f)) * g : 0.f;
+        *reinterpret_cast<float4*>(d + row * ldd + col) = out;
     }
 };
 
@@ -113,11 +392,11 @@ __global__ __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_pe
     using gemm::ppdev::kBand;
     if constexpr (WHAT == HeadTile::kLogSum) {
         half_gemm_pp_tile<BF16, false, true>(p, blockIdx.x, kBand,
-                                             LogSumEnd<8, 32>{h.rows, h.part, h.hit, h.parts, h.first_class});
+                                             LogSumEnd16{h.rows, h.part, h.hit, h.tokens, p.m, p.n, h.first_class});
     } else if constexpr (WHAT == HeadTile::kGradLogits) {
         half_gemm_pp_tile<BF16, false, true>(
             p, blockIdx.x, kBand,
-            GradLogitsEnd<T, 8>{h.rows, static_cast<T*>(h.d), h.ldd, (h.n + 7) & ~7, h.first_class});
+            GradLogitsEnd16<BF16>{h.rows, static_cast<T*>(h.d), h.ldd, p.m, p.n, (h.n + 7) & ~7, h.first_class});
     } else if constexpr (WHAT == HeadTile::kGradHidden) {
         const int first = blockIdx.z * h.k_chunk;
         p.a             = static_cast<const T*>(h.a) + first;
@@ -133,20 +412,58 @@ __global__ __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_pe
     }
 }
 
-template <HeadTile WHAT>
-__global__ __launch_bounds__(256, 2) void headTileFp32(HeadTileArgs h) {
-    gemm::GemmParams p{};
+// Three stage buffers: this tile runs where there are few workgroups to a CU (one needs two stages in
+// flight to be busy by itself).
+template <bool BF16, HeadTile WHAT>
+__global__ __launch_bounds__(256, 1) void headTileHalf128(HeadTileArgs h) {
+    using T = std::conditional_t<BF16, bf16, fp16>;
+    gemm::HalfGemmParams p{};
     if (!tileProblem<WHAT>(h, p, 128, 128)) return;
+    p.a = h.a, p.b = h.b, p.d = h.d;
+    using gemm::ddev::half_gemm_dma_tile;
+    using gemm::ddev::StoreTile;
+    if constexpr (WHAT == HeadTile::kLogSum) {
+        using End = LogSumEnd128;
+        half_gemm_dma_tile<BF16, false, true, 128, false, 128, 3, false, End>(
+            p, blockIdx.x, 0, 8, End{h.rows, h.part, h.hit, h.tokens, p.m, p.n, h.first_class});
+    } else if constexpr (WHAT == HeadTile::kGradLogits) {
+        using End = GradLogitsEnd128<BF16>;
+        half_gemm_dma_tile<BF16, false, true, 128, false, 128, 3, false, End>(
+            p, blockIdx.x, 0, 8, End{h.rows, static_cast<T*>(h.d), h.ldd, p.m, p.n, (h.n + 7) & ~7, h.first_class});
+    } else if constexpr (WHAT == HeadTile::kGradHidden) {
+        const int first = blockIdx.z * h.k_chunk;
+        p.a             = static_cast<const T*>(h.a) + first;
+        p.b             = static_cast<const T*>(h.b) + first * h.ldb;
+        p.k             = max(0, min(h.k_chunk, h.k - first));
+        p.d             = static_cast<float*>(h.d) + blockIdx.z * h.slice;
+        if (h.add) p.c = p.d;
+        half_gemm_dma_tile<BF16, false, false, 128, false, 128, 3>(p, blockIdx.x);
+    } else {
+        p.alpha   = h.head->inv_scale;
+        p.cd_half = 1;
+        half_gemm_dma_tile<BF16, true, false, 128, false, 128, 3>(p, blockIdx.x, 0, 8, StoreTile{}, h.read_m, h.read_n);
+    }
+}
+
+// FOLD 16: sums of 512 k.  An fp32 sum of all of k = 2048 .. 8192 in one chain left dl off by 6e-6 to
+// 1.5e-5 of its size (a logit of 16 is off by half a unit of 2^-20 at every step); folded, by 1.5e-6.  It
+// costs 5% on 2048 x 2048 x 32003 (5221 -> 5486 us for the gradients).
+template <HeadTile WHAT, int BM>
+__global__ __launch_bounds__(256, 2) void headTileFp32(HeadTileArgs h) {
+    constexpr int WM = BM == 128 ? 2 : 4, WN = BM == 128 ? 2 : 1, kFold = 16;
+    gemm::GemmParams p{};
+    if (!tileProblem<WHAT>(h, p, BM, BM)) return;
     p.a = static_cast<const float*>(h.a), p.b = static_cast<const float*>(h.b), p.d = static_cast<float*>(h.d);
     using gemm::d32::fp32_gemm_dma_tile;
     using gemm::d32::StoreTile;
-    constexpr int kFold = 16;
     if constexpr (WHAT == HeadTile::kLogSum) {
-        const LogSumEnd<4, 16> end{h.rows, h.part, h.hit, h.parts, h.first_class};
-        fp32_gemm_dma_tile<128, 128, 2, 2, false, true, false, false, decltype(end), kFold>(p, blockIdx.x, 0, 4, end);
+        using End = LogSumEnd32;
+        fp32_gemm_dma_tile<BM, BM, WM, WN, false, true, false, false, End, kFold>(
+            p, blockIdx.x, 0, 4, End{h.rows, h.part, h.hit, h.tokens, h.first_class});
     } else if constexpr (WHAT == HeadTile::kGradLogits) {
-        const GradLogitsEnd<float, 4> end{h.rows, static_cast<float*>(h.d), h.ldd, (h.n + 3) & ~3, h.first_class};
-        fp32_gemm_dma_tile<128, 128, 2, 2, false, true, false, false, decltype(end), kFold>(p, blockIdx.x, 0, 4, end);
+        using End = GradLogitsEnd32;
+        fp32_gemm_dma_tile<BM, BM, WM, WN, false, true, false, false, End, kFold>(
+            p, blockIdx.x, 0, 4, End{h.rows, static_cast<float*>(h.d), h.ldd, (h.n + 3) & ~3, h.first_class});
     } else if constexpr (WHAT == HeadTile::kGradHidden) {
         const int first = blockIdx.z * h.k_chunk;
         p.a += first;
@@ -154,36 +471,33 @@ __global__ __launch_bounds__(256, 2) void headTileFp32(HeadTileArgs h) {
         p.k = max(0, min(h.k_chunk, h.k - first));
         p.d += blockIdx.z * h.slice;
         if (h.add) p.c = p.d;
-        fp32_gemm_dma_tile<128, 128, 2, 2, false, false, false, false, StoreTile, kFold>(p, blockIdx.x, 0);
+        fp32_gemm_dma_tile<BM, BM, WM, WN, false, false, false, false, StoreTile, kFold>(p, blockIdx.x, 0);
     } else {
-        const GradWeightEnd end{static_cast<float*>(h.d), h.ldd};
-        fp32_gemm_dma_tile<128, 128, 2, 2, false, false, true, false, decltype(end), kFold>(p, blockIdx.x, 0, 4, end, h.read_m, h.read_n);
+        using End = GradWeightEnd;
+        fp32_gemm_dma_tile<BM, BM, WM, WN, false, false, true, false, End, kFold>(
+            p, blockIdx.x, 0, 4, End{static_cast<float*>(h.d), h.ldd}, h.read_m, h.read_n);
     }
 }
 
-inline dim3 headGrid(const HeadTileArgs& a, int size, int slices) {
+template <class K>
+void launchHead(K kernel, const char* name, const HeadTileArgs& a, int size, int threads, int slices, hipStream_t stream) {
     const int64_t tiles = (static_cast<int64_t>(a.m) + size - 1) / size * ((static_cast<int64_t>(a.n) + size - 1) / size);
     if (tiles > INT32_MAX) raise(FTRAIN_STATUS_UNSUPPORTED, "cross entropy: too many tiles (%lld)", (long long)tiles);
-    return dim3(static_cast<uint32_t>(tiles), 1, static_cast<uint32_t>(slices));
+    launch(kernel, name, dim3(static_cast<uint32_t>(tiles), 1, static_cast<uint32_t>(slices)), dim3(threads), stream, a);
 }
 
+constexpr const char* kHeadNames[4] = {"cross entropy logits", "cross entropy logits' gradient", "cross entropy hidden gradient",
+                                       "cross entropy weight gradient"};
+
 template <bool BF16>
-void launchHeadTileHalf(HeadTile what, const HeadTileArgs& args, int slices, hipStream_t stream) {
-    const dim3 grid = headGrid(args, 256, slices);
-    switch (what) {
-        case HeadTile::kLogSum:
-            launch(&headTileHalf<BF16, HeadTile::kLogSum>, "cross entropy logits", grid, dim3(512), stream, args);
-            break;
-        case HeadTile::kGradLogits:
-            launch(&headTileHalf<BF16, HeadTile::kGradLogits>, "cross entropy logits' gradient", grid, dim3(512), stream, args);
-            break;
-        case HeadTile::kGradHidden:
-            launch(&headTileHalf<BF16, HeadTile::kGradHidden>, "cross entropy hidden gradient", grid, dim3(512), stream, args);
-            break;
-        case HeadTile::kGradWeight:
-            launch(&headTileHalf<BF16, HeadTile::kGradWeight>, "cross entropy weight gradient", grid, dim3(512), stream, args);
-            break;
-    }
+void launchHeadTileHalf(HeadTile what, int size, const HeadTileArgs& args, int slices, hipStream_t stream) {
+    constexpr void (*large[4])(HeadTileArgs) = {&headTileHalf<BF16, HeadTile::kLogSum>, &headTileHalf<BF16, HeadTile::kGradLogits>,
+                                                &headTileHalf<BF16, HeadTile::kGradHidden>, &headTileHalf<BF16, HeadTile::kGradWeight>};
+    constexpr void (*small[4])(HeadTileArgs) = {
+        &headTileHalf128<BF16, HeadTile::kLogSum>, &headTileHalf128<BF16, HeadTile::kGradLogits>,
+        &headTileHalf128<BF16, HeadTile::kGradHidden>, &headTileHalf128<BF16, HeadTile::kGradWeight>};
+    const int i = static_cast<int>(what);
+    launchHead(size == 256 ? large[i] : small[i], kHeadNames[i], args, size, size == 256 ? 512 : 256, slices, stream);
 }
 
 }  // namespace ftrain::train
