@@ -12,10 +12,6 @@
 
 namespace ftrain::train {
 
-// exp(x) as 2^(x log2 e): the product's rounding is off by |x| 2^-24 of the result, less than what the
-// logits' own sums are.
-__device__ __forceinline__ float expFast(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
-
 // ---- 16-bit operands: the 256x256 tile of gemm/pingpong_tile.hpp.
 //
 // A lane holds, of row 128 i + 64 wm + 16 u + j16 of the tile, columns 128 j + 32 wn + 16 v + 4 g + r

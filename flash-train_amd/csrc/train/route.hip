@@ -9,8 +9,11 @@
 //   dp_te = gl E f_e / N + [e chosen] dgate, dl_t = p_t (dp_t - sum_e p_te dp_te)
 // and with normalised gates w the chosen entries' part is w (dgate - sum w dgate) instead.
 //
-// A group of G lanes owns a row, eight logits in each lane (16 above 512 experts): softmax and
-// selection stay in registers and cross the group by lane shuffles.  A workgroup takes a run of
+// A group of G lanes owns a row, eight logits in each lane (16 above 128 experts): softmax and selection
+// stay in registers and cross the group by lane permutations.  With many experts vector instructions
+// bound the choice, 131072 x 256 fp32, top 8: pairs of value and index reduced by shuffles 148 us,
+// maxima first and then the place by a ballot 109, on whole numbers 87 (eight a lane), 59 (16 a lane: the
+// steps across lanes serve four rows of a wave instead of two).  A workgroup takes a run of
 // consecutive rows, so the order of the choices within an expert is the order of (workgroup, row,
 // rank): `choose` counts each workgroup's choices, `scan` turns them into each workgroup's first
 // rank (one workgroup per expert), `place` hands out the slots.  Sums over rows are taken in a fixed
@@ -25,8 +28,13 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves   = kThreads / kWave;
-// Most workgroups: four on each of the 256 CUs.
-constexpr int kMaxBlocks = 1024;
+constexpr int kCus     = 256;
+// Most workgroups.
+constexpr int kMaxBlocks = 4 * kCus;
+// Which form the forward pass takes (moeRouteForward): passes of one workgroup over rows, and counts.
+constexpr uint64_t kWholePasses = 4, kScanPasses = 8, kScanCounts = 32768;
+// Workgroups of the form without `scan`.
+constexpr int kMidBlocks = kCus;
 
 struct RouteArgs {
     const void* logits;
@@ -38,7 +46,7 @@ struct RouteArgs {
     int64_t rows, ld, grad_ld;
     int32_t n_experts, top_k, rows_per_block, blocks;
     int32_t normalize;
-    // Workspace: of each expert, each workgroup's choices (then their first rank) and sum of p; of
+    // Workspace: of each workgroup and expert, the choices (then their first rank) and the sum of p; of
     // each workgroup, its routed rows; of each expert, its sum of p.
     int32_t* block_count;
     float* block_p;
@@ -54,6 +62,10 @@ struct Row {
     int g;
 
     __device__ __forceinline__ int index(int j) const { return VEC ? g * VPL + j : g + G * j; }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) v[j] = -INFINITY;
+    }
     __device__ __forceinline__ void load(const T* row, int n) {
         if constexpr (VEC) {
             constexpr int N = 16 / sizeof(T);
@@ -74,36 +86,124 @@ struct Row {
             for (int j = 0; j < VPL; ++j) v[j] = index(j) < n ? toFloat(row[index(j)]) : -INFINITY;
         }
     }
-    // Exponentials relative to the largest logit into p; their sum is returned.  any: some logit is
-    // not minus infinity.
-    __device__ __forceinline__ float exponentials(float (&p)[VPL], float& top, bool& any) const {
-        float m = -INFINITY;
-        int some = 0;
+    // Exponentials relative to `top` into p; their sum is returned: 0 only where every logit is minus
+    // infinity (a NaN makes it NaN).
+    __device__ __forceinline__ float exponentials(float (&p)[VPL], float top) const {
+        const float base = top == -INFINITY ? 0.f : top;
+        float total      = 0.f;
 #pragma unroll
         for (int j = 0; j < VPL; ++j) {
-            m = fmaxf(m, v[j]);
-            some |= v[j] != -INFINITY;
-        }
-        top = groupMax<G>(m);
-#pragma unroll
-        for (int d = 1; d < G; d <<= 1) some |= __shfl_xor(some, d, kWave);
-        any         = some != 0;
-        float total = 0.f;
-#pragma unroll
-        for (int j = 0; j < VPL; ++j) {
-            p[j] = expf(v[j] - top);
+            p[j] = expFast(v[j] - base);
             total += p[j];
         }
         return groupSum<G>(total);
     }
+    __device__ __forceinline__ float largest() const {
+        float m = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) m = fmaxf(m, v[j]);
+        return groupMax<G>(m);
+    }
+};
+
+__device__ __forceinline__ unsigned maxOf(unsigned a, unsigned b) { return a > b ? a : b; }
+
+// The logits as whole numbers in their order, from which the largest are taken one by one (0: taken; a
+// NaN counts as minus infinity, which is never chosen; the two zeros are one).  Integers, because a
+// floating maximum of values that may be NaN takes two more instructions to make them quiet, at every
+// step.
+//   A 16-bit logit leaves 13 bits of its number free: they hold 1023 less its index, so the largest
+// number is the largest logit with the lowest index, and nothing else need be found out.
+template <class T, int VPL, int G, bool VEC>
+struct Candidates {
+    static constexpr bool kPacked    = sizeof(T) == 2;
+    static constexpr unsigned kIndex = kMaxExperts - 1, kFree = 0x1FFFu;
+    static constexpr unsigned kLeast = 0x00800000u;  // the number of the lowest finite value is not less
+    unsigned key[VPL];
+
+    __device__ __forceinline__ explicit Candidates(const Row<T, VPL, G, VEC>& row) {
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+            const unsigned bits = __builtin_bit_cast(unsigned, fmaxf(row.v[j] + 0.f, -INFINITY));
+            unsigned k          = bits ^ (static_cast<unsigned>(static_cast<int>(bits) >> 31) | 0x80000000u);
+            if constexpr (kPacked) k = (k & ~kFree) | (kIndex - row.index(j));
+            key[j] = k;
+        }
+    }
+    __device__ __forceinline__ unsigned mine() const {
+        unsigned m = key[0];
+#pragma unroll
+        for (int j = 1; j < VPL; ++j) m = maxOf(m, key[j]);
+        return m;
+    }
+    // The group's largest number.
+    __device__ __forceinline__ unsigned best(unsigned own) const {
+        return groupReduce<G>(own, [](unsigned a, unsigned b) { return maxOf(a, b); });
+    }
+    static __device__ __forceinline__ float value(unsigned k) {
+        if (k < kLeast) return -INFINITY;
+        if constexpr (kPacked) k = (k & 0x80000000u) ? k & ~kFree : k | kFree;
+        return __builtin_bit_cast(float, (k & 0x80000000u) ? k ^ 0x80000000u : ~k);
+    }
+    // Takes out the largest, `best`; returns its index.  own: mine().
+    __device__ __forceinline__ int take(unsigned best, unsigned own, const Row<T, VPL, G, VEC>& row) {
+        if constexpr (kPacked) {
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) key[j] = key[j] == best ? 0u : key[j];
+            return kIndex - (best & kIndex);
+        } else if constexpr (VEC) {
+            // Lanes hold their logits in the row's order: of those that tie, the lowest lane has the
+            // lowest index.
+            bool open = own == best;
+            int from  = 0;
+            if constexpr (G > 1) {
+                const unsigned long long all = __ballot(open);
+                const int lane = threadIdx.x % kWave, first = lane - row.g;
+                const unsigned long long group = G == kWave ? all : (all >> first) & ((1ull << (G % kWave)) - 1ull);
+                from = first + __builtin_ctzll(group);
+                open = open && from == lane;
+            }
+            int found = 0;
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) {
+                const bool hit = open && key[j] == best;
+                found          = hit ? row.index(j) : found;
+                key[j]         = hit ? 0u : key[j];
+                open           = open && !hit;
+            }
+            return G > 1 ? __shfl(found, from, kWave) : found;
+        } else {
+            int found = INT32_MAX;
+#pragma unroll
+            for (int j = VPL - 1; j >= 0; --j)
+                if (key[j] == best) found = row.index(j);
+            const int at = groupReduce<G>(found, [](int a, int b) { return min(a, b); });
+#pragma unroll
+            for (int j = 0; j < VPL; ++j)
+                if (row.index(j) == at) key[j] = 0u;
+            return at;
+        }
+    }
+};
+
+// What `choose` and `place` keep in LDS, one after the other.
+union RouteLds {
+    struct {
+        int hist[kMaxExperts];
+        float sums[kThreads * 16];
+        int routed[kThreads];
+    } choose;
+    struct {
+        int first[kMaxExperts];         // slot of the workgroup's first choice of each expert
+        int next[kWaves][kMaxExperts];  // each wave's choices, then its next slot
+    } place;
 };
 
 template <class T, int VPL, int G, bool VEC>
-__global__ __launch_bounds__(kThreads) void choose(RouteArgs a) {
+__device__ __forceinline__ void chooseRows(const RouteArgs& a, RouteLds& lds) {
     constexpr int kRows = kThreads / G;  // rows at a time
-    __shared__ int hist[kMaxExperts];
-    __shared__ float sums[kThreads * VPL];
-    __shared__ int routed_of[kRows];
+    int* const hist   = lds.choose.hist;
+    float* const sums = lds.choose.sums;
     const int group = threadIdx.x / G, n = a.n_experts;
     Row<T, VPL, G, VEC> row;
     row.g = threadIdx.x % G;
@@ -118,13 +218,16 @@ __global__ __launch_bounds__(kThreads) void choose(RouteArgs a) {
         const bool kept = a.mask == nullptr || a.mask[t] != 0;
         int32_t* const experts = a.experts + t * a.top_k;
         float* const gates     = a.gates + t * a.top_k;
-        float p[VPL], top = 0.f, total = 1.f;
-        bool any = false;
-        if (kept) {
+        if (kept)
             row.load(static_cast<const T*>(a.logits) + t * a.ld, n);
-            total = row.exponentials(p, top, any);
-        }
-        if (!any) {
+        else
+            row.clear();
+        Candidates<T, VPL, G, VEC> left(row);
+        unsigned own = left.mine(), best = left.best(own);
+        const float top = left.value(best);
+        float p[VPL];
+        const float total = row.exponentials(p, top);
+        if (total == 0.f) {
             for (int k = row.g; k < a.top_k; k += G) {
                 experts[k] = -1;
                 gates[k]   = 0.f;
@@ -133,51 +236,56 @@ __global__ __launch_bounds__(kThreads) void choose(RouteArgs a) {
         }
         const float inv = 1.f / total;
 #pragma unroll
-        for (int j = 0; j < VPL; ++j) sum_p[j] += row.index(j) < n ? p[j] * inv : 0.f;
+        for (int j = 0; j < VPL; ++j) sum_p[j] += p[j] * inv;
         ++routed;
-        float chosen = 0.f;  // sum of the chosen p
-        float gate   = 0.f;  // lane k % G keeps the gates k, k + G ..: written at once below
-        for (int k = 0; k < a.top_k; ++k) {
-            float best = -INFINITY;
-            int at     = n;
+        // Lane g keeps choices g, g + G ..
+        constexpr int kSlots = VPL < kMaxTopK / G ? VPL : G < kMaxTopK ? kMaxTopK / G : 1;
+        float gate[kSlots], chosen = 0.f;
+        int at[kSlots];
 #pragma unroll
-            for (int j = 0; j < VPL; ++j)
-                if (row.v[j] > best) best = row.v[j], at = row.index(j);
-#pragma unroll
-            for (int d = 1; d < G; d <<= 1) {
-                const float other = __shfl_xor(best, d, kWave);
-                const int oat     = __shfl_xor(at, d, kWave);
-                if (other > best || (other == best && oat < at)) best = other, at = oat;
+        for (int s = 0; s < kSlots; ++s) {
+            at[s]   = INT32_MAX;
+            gate[s] = 0.f;
+            if (s * G >= a.top_k) continue;
+            unsigned number = 0;
+            for (int k = 0; k < G && s * G + k < a.top_k; ++k) {
+                const int e = left.take(best, own, row);
+                if (k == row.g) at[s] = best >= left.kLeast ? e : INT32_MAX, number = best;
+                own  = left.mine();
+                best = left.best(own);
             }
-            const bool found = at < n;
-#pragma unroll
-            for (int j = 0; j < VPL; ++j)
-                if (row.index(j) == at) row.v[j] = -INFINITY;
             // A row whose sum is NaN has NaN gates.
-            gate = found ? expf(best - top) * inv : 0.f;
-            chosen += gate;
-            if (row.g == 0) {
-                experts[k] = found ? at : -1;
-                gates[k]   = gate;
-                if (found) atomicAdd(&hist[at], 1);
+            gate[s] = at[s] < n ? expExact(left.value(number) - top) * inv : 0.f;
+            chosen += gate[s];
+        }
+        if (a.normalize) {
+            const float scale = 1.f / groupSum<G>(chosen);
+#pragma unroll
+            for (int s = 0; s < kSlots; ++s) gate[s] = at[s] < n ? gate[s] * scale : 0.f;
+        }
+#pragma unroll
+        for (int s = 0; s < kSlots; ++s) {
+            const int k = s * G + row.g;
+            if (k < a.top_k) {
+                experts[k] = at[s] < n ? at[s] : -1;
+                gates[k]   = gate[s];
+                if (at[s] < n) atomicAdd(&hist[at[s]], 1);
             }
         }
-        if (a.normalize && row.g == 0)
-            for (int k = 0; k < a.top_k; ++k) gates[k] = experts[k] >= 0 ? gates[k] / chosen : 0.f;
     }
 #pragma unroll
     for (int j = 0; j < VPL; ++j) sums[group * (G * VPL) + row.index(j)] = sum_p[j];
-    if (row.g == 0) routed_of[group] = routed;
+    if (row.g == 0) lds.choose.routed[group] = routed;
     __syncthreads();
     for (int e = threadIdx.x; e < n; e += kThreads) {
         float s = 0.f;
         for (int r = 0; r < kRows; ++r) s += sums[r * (G * VPL) + e];
-        a.block_count[static_cast<int64_t>(e) * a.blocks + blockIdx.x] = hist[e];
-        a.block_p[static_cast<int64_t>(e) * a.blocks + blockIdx.x]     = s;
+        a.block_count[static_cast<int64_t>(blockIdx.x) * n + e] = hist[e];
+        a.block_p[static_cast<int64_t>(blockIdx.x) * n + e]     = s;
     }
     if (threadIdx.x == 0) {
         int s = 0;
-        for (int r = 0; r < kRows; ++r) s += routed_of[r];
+        for (int r = 0; r < kRows; ++r) s += lds.choose.routed[r];
         a.block_routed[blockIdx.x] = s;
     }
 }
@@ -205,51 +313,128 @@ __device__ __forceinline__ int blockScan(int v, int& total) {
     return before + s - v;
 }
 
-// Expert blockIdx.x: each workgroup's first rank in place of its count, the expert's count, its sum of p.
+// Of kScanExperts experts: each workgroup's first rank in place of its count, the expert's count, its sum
+// of p.  Adjacent threads take adjacent experts, each a run of the workgroups.
+constexpr int kScanExperts = 8;
 __global__ __launch_bounds__(kThreads) void scan(RouteArgs a) {
-    int32_t* const count = a.block_count + static_cast<int64_t>(blockIdx.x) * a.blocks;
-    const float* const p = a.block_p + static_cast<int64_t>(blockIdx.x) * a.blocks;
-    __shared__ float part[kWaves];
-    int before = 0;
-    float sum  = 0.f;
-    for (int b0 = 0; b0 < a.blocks; b0 += kThreads) {
-        const int b  = b0 + threadIdx.x;
-        const bool in = b < a.blocks;
-        int total;
-        const int at = blockScan(in ? count[b] : 0, total);
-        if (in) {
-            count[b] = before + at;
-            sum += p[b];
-        }
-        before += total;
+    constexpr int kRuns = kThreads / kScanExperts;
+    __shared__ int counts[kRuns][kScanExperts];
+    __shared__ float sums[kRuns][kScanExperts];
+    const int n = a.n_experts, run = threadIdx.x / kScanExperts, i = threadIdx.x % kScanExperts;
+    const int e = blockIdx.x * kScanExperts + i, per = (a.blocks + kRuns - 1) / kRuns;
+    const int first = run * per, last = e < n ? min(first + per, a.blocks) : first;
+    int32_t* const count = a.block_count + e;
+    const float* const p = a.block_p + e;
+    int c                = 0;
+    float sum            = 0.f;
+#pragma unroll 8
+    for (int b = first; b < last; ++b) {
+        c += count[static_cast<int64_t>(b) * n];
+        sum += p[static_cast<int64_t>(b) * n];
     }
-    sum = groupSum<kWave>(sum);
-    if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = sum;
+    counts[run][i] = c;
+    sums[run][i]   = sum;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kWaves; ++w) sum += part[w];
-        a.counts[blockIdx.x] = before;
-        a.sum_p[blockIdx.x]  = sum;
+    int before = 0;
+    for (int r = 0; r < run; ++r) before += counts[r][i];
+    if (run == kRuns - 1 && e < n) {
+        float all = 0.f;
+        for (int r = 0; r < kRuns; ++r) all += sums[r][i];
+        a.counts[e] = before + c;
+        a.sum_p[e]  = all;
+    }
+#pragma unroll 8
+    for (int b = first; b < last; ++b) {
+        const int x                         = count[static_cast<int64_t>(b) * n];
+        count[static_cast<int64_t>(b) * n] = before;
+        before += x;
     }
 }
 
-// The slots of the workgroup's choices; workgroup 0 also finishes the loss.
-__global__ __launch_bounds__(kThreads) void place(RouteArgs a) {
-    __shared__ int first[kMaxExperts];            // slot of the workgroup's first choice of each expert
-    __shared__ int next[kWaves][kMaxExperts];     // each wave's choices, then its next slot
+// The slots of the workgroup's choices; workgroup 0 also finishes the loss.  SCANNED: `scan` has run;
+// else every workgroup adds up the others' counts by itself.
+template <bool SCANNED>
+__device__ __forceinline__ void placeRows(const RouteArgs& a, RouteLds& lds) {
+    int* const first = lds.place.first;
+    auto& next       = lds.place.next;
     const int n = a.n_experts, lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    if constexpr (!SCANNED) {
+        // A thread an expert, or several: adjacent threads adjacent experts, each with the workgroups
+        // from `part` on in steps of `parts`.
+        const int parts = n <= kThreads / 4 ? 4 : n <= kThreads / 2 ? 2 : 1;
+        const int part = threadIdx.x / (kThreads / parts), self = blockIdx.x;
+        __shared__ int all_of[kThreads], before_of[kThreads];
+        __shared__ float sum_of[kThreads];
+        for (int e0 = 0; e0 < n; e0 += kThreads / parts) {
+            const int e = e0 + threadIdx.x % (kThreads / parts);
+            int all = 0, before = 0;
+            float sum = 0.f;
+            if (e < n) {
+#pragma unroll 16
+                for (int b = part; b < a.blocks; b += parts) {
+                    const int c = a.block_count[static_cast<int64_t>(b) * n + e];
+                    all += c;
+                    before += b < self ? c : 0;
+                }
+                if (self == 0) {
+#pragma unroll 16
+                    for (int b = part; b < a.blocks; b += parts) sum += a.block_p[static_cast<int64_t>(b) * n + e];
+                }
+            }
+            all_of[threadIdx.x]    = all;
+            before_of[threadIdx.x] = before;
+            sum_of[threadIdx.x]    = sum;
+            __syncthreads();
+            if (part == 0 && e < n) {
+                for (int q = 1; q < parts; ++q) {
+                    all += all_of[threadIdx.x + q * (kThreads / parts)];
+                    before += before_of[threadIdx.x + q * (kThreads / parts)];
+                    sum += sum_of[threadIdx.x + q * (kThreads / parts)];
+                }
+                next[0][e] = all;
+                next[1][e] = before;
+                next[2][e] = __builtin_bit_cast(int, sum);
+                if (self == 0) a.counts[e] = all;
+            }
+            __syncthreads();
+        }
+    }
+    auto count_of = [&](int e) { return SCANNED ? a.counts[e] : next[0][e]; };
+    if (blockIdx.x == 0) {
+        __shared__ float part[kWaves];
+        int routed = 0, total = 0;
+        for (int b = threadIdx.x; b < a.blocks; b += kThreads) routed += a.block_routed[b];
+        float dot = 0.f;
+        for (int e = threadIdx.x; e < n; e += kThreads) {
+            const int c = count_of(e);
+            total += c;
+            dot += static_cast<float>(c) * (SCANNED ? a.sum_p[e] : __builtin_bit_cast(float, next[2][e]));
+        }
+        int all_routed, all;
+        (void)blockScan(routed, all_routed);
+        (void)blockScan(total, all);
+        dot = groupSum<kWave>(dot);
+        if (lane == 0) part[wave] = dot;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int w = 1; w < kWaves; ++w) dot += part[w];
+            *a.routed = all_routed;
+            *a.loss   = static_cast<float>(n) * (dot / static_cast<float>(max(all, 1))) / static_cast<float>(max(all_routed, 1));
+        }
+    }
     int before = 0;
     for (int e0 = 0; e0 < n; e0 += kThreads) {
         const int e = e0 + threadIdx.x;
         int total;
-        const int at = blockScan(e < n ? a.counts[e] : 0, total);
-        if (e < n) first[e] = before + at;
+        const int at = blockScan(e < n ? count_of(e) : 0, total);
+        if (e < n)
+            first[e] = before + at +
+                       (SCANNED ? a.block_count[static_cast<int64_t>(blockIdx.x) * n + e] : next[1][e]);
         before += total;
     }
-    for (int e = threadIdx.x; e < n; e += kThreads) {
-        first[e] += a.block_count[static_cast<int64_t>(e) * a.blocks + blockIdx.x];
+    __syncthreads();
+    for (int e = threadIdx.x; e < n; e += kThreads)
         for (int w = 0; w < kWaves; ++w) next[w][e] = 0;
-    }
     __syncthreads();
     const int64_t begin = static_cast<int64_t>(blockIdx.x) * a.rows_per_block * a.top_k;
     const int64_t end   = min(begin + static_cast<int64_t>(a.rows_per_block) * a.top_k, a.rows * a.top_k);
@@ -279,48 +464,43 @@ __global__ __launch_bounds__(kThreads) void place(RouteArgs a) {
             peers &= (e & bit) ? set : ~set;
         }
         int slot = -1;
-        if (e >= 0) {
-            const int rank = __popcll(peers & ((1ull << lane) - 1ull));
-            slot           = next[wave][e] + rank;
-        }
+        if (e >= 0) slot = next[wave][e] + __popcll(peers & ((1ull << lane) - 1ull));
         // Every lane has read before the last of each expert's lanes writes, and the next round reads
-        // after it: one wave's LDS accesses are done in order.
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        // after it.
+        waveFence();
         if (e >= 0 && (peers >> lane) == 1ull) next[wave][e] = slot + 1;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        waveFence();
         if (i < stop) a.slots[i] = slot;
     }
+}
 
-    if (blockIdx.x != 0) return;
-    __shared__ float part[kWaves];
-    int routed = 0, total = 0;
-    for (int b = threadIdx.x; b < a.blocks; b += kThreads) routed += a.block_routed[b];
-    float dot = 0.f;
-    for (int e = threadIdx.x; e < n; e += kThreads) {
-        total += a.counts[e];
-        dot += static_cast<float>(a.counts[e]) * a.sum_p[e];
-    }
-    int all_routed, all;
-    (void)blockScan(routed, all_routed);
-    (void)blockScan(total, all);
-    dot = groupSum<kWave>(dot);
-    if (lane == 0) part[wave] = dot;
+// One workgroup that has all rows goes on to place them.
+template <class T, int VPL, int G, bool VEC>
+__global__ __launch_bounds__(kThreads) void choose(RouteArgs a) {
+    __shared__ RouteLds lds;
+    chooseRows<T, VPL, G, VEC>(a, lds);
+    if (a.blocks > 1) return;
+    // The workgroup's own stores are there for it after the barrier.
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kWaves; ++w) dot += part[w];
-        *a.routed = all_routed;
-        *a.loss   = static_cast<float>(n) * (dot / static_cast<float>(max(all, 1))) / static_cast<float>(max(all_routed, 1));
-    }
+    placeRows<false>(a, lds);
+}
+
+template <bool SCANNED>
+__global__ __launch_bounds__(kThreads) void place(RouteArgs a) {
+    __shared__ RouteLds lds;
+    placeRows<SCANNED>(a, lds);
 }
 
 template <class T, int VPL, int G, bool VEC>
 __global__ __launch_bounds__(kThreads) void backward(RouteArgs a) {
     constexpr int kRows = kThreads / G;
+    // Of each group's row: p, and what its choices add to the gradient.
+    __shared__ __attribute__((aligned(16))) float row_p[kThreads * VPL], row_add[kThreads * VPL];
     const int group = threadIdx.x / G, n = a.n_experts;
     Row<T, VPL, G, VEC> row;
-    row.g = threadIdx.x % G;
+    row.g              = threadIdx.x % G;
+    float* const all_p = row_p + group * (G * VPL);
+    float* const add   = row_add + group * (G * VPL);
     int total = 0, all;
     for (int e = threadIdx.x; e < n; e += kThreads) total += a.counts[e];
     (void)blockScan(total, all);
@@ -335,63 +515,53 @@ __global__ __launch_bounds__(kThreads) void backward(RouteArgs a) {
     const int64_t stride = static_cast<int64_t>(gridDim.x) * kRows;
     for (int64_t t = static_cast<int64_t>(blockIdx.x) * kRows + group; t < a.rows; t += stride) {
         T* const out = static_cast<T*>(a.grad_logits) + t * a.grad_ld;
-        float p[VPL], d[VPL], top, inv = 0.f;
-        bool any = false;
+        float p[VPL], d[VPL] = {}, sum = 0.f;
         if (a.mask == nullptr || a.mask[t] != 0) {
             row.load(static_cast<const T*>(a.logits) + t * a.ld, n);
-            inv = 1.f / row.exponentials(p, top, any);
+            sum = row.exponentials(p, row.largest());
         }
-        if (any) {
+        if (sum != 0.f) {
             const int32_t* const experts = a.experts + t * a.top_k;
             const float* const grads     = a.grad_gates + t * a.top_k;
-            float dot = 0.f;
+            const float inv              = 1.f / sum;
+            // The choices reach their experts' lanes through LDS (a comparison of every choice with
+            // every logit took most of the kernel: 100003 x 160, six choices, 46 -> 33 us).
 #pragma unroll
             for (int j = 0; j < VPL; ++j) {
-                p[j] = row.index(j) < n ? p[j] * inv : 0.f;
-                d[j] = balance[j];
+                p[j] *= inv;
+                add[row.index(j)] = 0.f;
+                if (a.normalize) all_p[row.index(j)] = p[j];
             }
+            waveFence();
+            float picked = 0.f, weighted = 0.f;
             if (a.normalize) {
-                // Of the chosen: sum of p, and sum of p dgate; both over the group.
-                float picked = 0.f, weighted = 0.f, dg[VPL] = {};
-                unsigned is = 0;
-                for (int k = 0; k < a.top_k; ++k) {
-                    const int e     = experts[k];
-                    const float dgk = grads[k];
-#pragma unroll
-                    for (int j = 0; j < VPL; ++j)
-                        if (row.index(j) == e) {
-                            dg[j] = dgk;
-                            is |= 1u << j;
-                            picked += p[j];
-                            weighted += p[j] * dgk;
-                        }
+                // Of the chosen: sum of p, and sum of p dgate.
+                for (int k = row.g; k < a.top_k; k += G) {
+                    const int e = experts[k];
+                    if (e >= 0 && e < n) {
+                        picked += all_p[e];
+                        weighted += all_p[e] * grads[k];
+                    }
                 }
                 picked   = groupSum<G>(picked);
                 weighted = groupSum<G>(weighted);
-#pragma unroll
-                for (int j = 0; j < VPL; ++j) dot += p[j] * d[j];
-                dot = groupSum<G>(dot);
-                const float mean = weighted / picked;
-#pragma unroll
-                for (int j = 0; j < VPL; ++j)
-                    d[j] = p[j] * (d[j] - dot) + ((is >> j) & 1u ? p[j] / picked * (dg[j] - mean) : 0.f);
-            } else {
-                for (int k = 0; k < a.top_k; ++k) {
-                    const int e     = experts[k];
-                    const float dgk = grads[k];
-#pragma unroll
-                    for (int j = 0; j < VPL; ++j)
-                        if (row.index(j) == e) d[j] += dgk;
-                }
-#pragma unroll
-                for (int j = 0; j < VPL; ++j) dot += p[j] * d[j];
-                dot = groupSum<G>(dot);
-#pragma unroll
-                for (int j = 0; j < VPL; ++j) d[j] = p[j] * (d[j] - dot);
             }
-        } else {
+            for (int k = row.g; k < a.top_k; k += G) {
+                const int e = experts[k];
+                if (e >= 0 && e < n) add[e] = a.normalize ? all_p[e] / picked * (grads[k] - weighted / picked) : grads[k];
+            }
+            waveFence();
+            float dot = 0.f, more[VPL];
 #pragma unroll
-            for (int j = 0; j < VPL; ++j) d[j] = 0.f;
+            for (int j = 0; j < VPL; ++j) {
+                more[j] = add[row.index(j)];
+                d[j]    = a.normalize ? balance[j] : balance[j] + more[j];
+                dot += p[j] * d[j];
+            }
+            waveFence();
+            dot = groupSum<G>(dot);
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) d[j] = p[j] * (d[j] - dot) + (a.normalize ? more[j] : 0.f);
         }
         if constexpr (VEC) {
             constexpr int N = 16 / sizeof(T);
@@ -425,14 +595,22 @@ Kernel kernelFor(int n, int& lanes) {
     };
     using std::integral_constant;
     const integral_constant<int, 8> eight;
+    const integral_constant<int, 16> sixteen;
     if (n <= 8) return pick(integral_constant<int, 1>{}, eight);
     if (n <= 16) return pick(integral_constant<int, 2>{}, eight);
     if (n <= 32) return pick(integral_constant<int, 4>{}, eight);
     if (n <= 64) return pick(integral_constant<int, 8>{}, eight);
     if (n <= 128) return pick(integral_constant<int, 16>{}, eight);
-    if (n <= 256) return pick(integral_constant<int, 32>{}, eight);
-    if (n <= 512) return pick(integral_constant<int, 64>{}, eight);
-    return pick(integral_constant<int, 64>{}, integral_constant<int, 16>{});
+    // Backward has no steps across lanes to share, and is bound by memory with eight a lane (100003 x 160
+    // fp32: 33 us, with 16 a lane 45).
+    if constexpr (BACK) {
+        if (n <= 256) return pick(integral_constant<int, 32>{}, eight);
+        if (n <= 512) return pick(integral_constant<int, 64>{}, eight);
+    } else {
+        if (n <= 256) return pick(integral_constant<int, 16>{}, sixteen);
+        if (n <= 512) return pick(integral_constant<int, 32>{}, sixteen);
+    }
+    return pick(integral_constant<int, 64>{}, sixteen);
 }
 
 template <bool BACK>
@@ -485,9 +663,16 @@ void moeRouteForward(const MoeRoute& p, void* workspace, hipStream_t stream) {
     int lanes   = 0;
     const Kernel kernel =
         kernelFor<false>(p.type, vectorRows(p.logits, p.type), static_cast<int>(p.logits.cols), lanes);
-    // Whole passes of the workgroup, at most kMaxBlocks workgroups.
-    const uint64_t at_once = kThreads / lanes;
-    const uint64_t passes  = std::max<uint64_t>(1, ceilDiv(ceilDiv(a.rows, at_once), kMaxBlocks));
+    // Whole passes of the workgroup over its rows, in one of three forms:
+    //   few passes in all: one workgroup does everything, in one launch (64 x 8: 15.8 us in three
+    //     launches, 9.0 in one);
+    //   as many workgroups as CUs, while the counts that each of `place` then reads (one of every
+    //     workgroup and expert) stay few: two launches (16384 x 64: 15.2 us in three, 13.5 in two);
+    //   four workgroups on each CU, and `scan` between.
+    const uint64_t at_once = kThreads / lanes, all = ceilDiv(a.rows, at_once);
+    const bool whole       = all <= kWholePasses;
+    const bool scanned     = !whole && (all > kScanPasses * kMidBlocks || p.logits.cols * kMidBlocks > kScanCounts);
+    const uint64_t passes  = whole ? std::max<uint64_t>(1, all) : ceilDiv(all, scanned ? kMaxBlocks : kMidBlocks);
     a.rows_per_block       = static_cast<int32_t>(passes * at_once);
     a.blocks               = static_cast<int32_t>(std::max<uint64_t>(1, ceilDiv(a.rows, a.rows_per_block)));
     a.block_count          = static_cast<int32_t*>(workspace);
@@ -495,8 +680,13 @@ void moeRouteForward(const MoeRoute& p, void* workspace, hipStream_t stream) {
     a.block_routed         = reinterpret_cast<int32_t*>(a.block_p + p.logits.cols * kMaxBlocks);
     a.sum_p                = reinterpret_cast<float*>(a.block_routed + kMaxBlocks);
     launch(kernel, "router choose", dim3(a.blocks), dim3(kThreads), stream, a);
-    launch(&scan, "router scan", dim3(a.n_experts), dim3(kThreads), stream, a);
-    launch(&place, "router place", dim3(a.blocks), dim3(kThreads), stream, a);
+    if (a.blocks == 1) return;
+    if (scanned) {
+        launch(&scan, "router scan", dim3(static_cast<uint32_t>(ceilDiv(a.n_experts, kScanExperts))), dim3(kThreads), stream, a);
+        launch(&place<true>, "router place", dim3(a.blocks), dim3(kThreads), stream, a);
+    } else {
+        launch(&place<false>, "router place", dim3(a.blocks), dim3(kThreads), stream, a);
+    }
 }
 
 void moeRouteBackward(const MoeRoute& p, hipStream_t stream) {
