@@ -210,9 +210,9 @@ uint64_t roundUp(uint64_t a, uint64_t b) { return ceilDiv(a, b) * b; }
 constexpr uint64_t kPieceBytes = 256ull << 20;
 constexpr uint64_t kCus = 256;
 
-// How a product runs: tile rows and columns, and slices of k that keep sums of their own.
+// How a product runs: tile rows (launchHeadTile), and slices of k that keep sums of their own.
 struct Tiling {
-    int size;
+    int rows;
     int slices;
 };
 
@@ -231,18 +231,24 @@ double tileMicros(bool fp32, int size, int64_t m, int64_t n, int64_t k, int slic
     return static_cast<double>(rounds) * (static_cast<double>(ceilDiv(k, slices)) / (fp32 ? 32 : 64) * stage + ends);
 }
 
-// sliced: k may be cut until the tiles fill the device (two fp32 workgroups run on a CU), in slices of
-// at least 512.
-Tiling tilingOf(FTrainNumericType type, int64_t m, int64_t n, int64_t k, bool sliced) {
-    const bool fp32 = type == FTRAIN_NUMERIC_TYPE_FP32;
+// sliced: k may be cut until the tiles fill the device (two workgroups of fp32 and of the 64x128 tile run
+// on a CU), in slices of at least 512.
+Tiling tilingOf(FTrainNumericType type, HeadTile what, int64_t m, int64_t n, int64_t k) {
+    const bool fp32 = type == FTRAIN_NUMERIC_TYPE_FP32, sliced = what == HeadTile::kGradHidden;
+    auto slicesOf = [&](int rows, int cols, int at_once) {
+        const uint64_t tiles = std::max<uint64_t>(1, ceilDiv(m, rows) * ceilDiv(n, cols));
+        return sliced ? static_cast<int>(std::max<uint64_t>(1, std::min<uint64_t>(at_once * kCus / tiles, k / 512))) : 1;
+    };
+    // The rows of the weight's gradient are the classes: many, and fp32 has the large tile only.
+    if (fp32 && what == HeadTile::kGradWeight) return {128, 1};
+    // At most 64 tokens: 16x4096x32003 bf16 loss @FEW@.
+    if (!fp32 && what != HeadTile::kGradWeight && m <= 64) return {64, slicesOf(64, 128, 2)};
     Tiling best{};
     double least = 0.0;
     for (const int size : {fp32 ? 128 : 256, fp32 ? 64 : 128}) {
-        const uint64_t tiles = std::max<uint64_t>(1, ceilDiv(m, size) * ceilDiv(n, size));
-        int slices           = 1;
-        if (sliced) slices = static_cast<int>(std::max<uint64_t>(1, std::min<uint64_t>((fp32 ? 2 : 1) * kCus / tiles, k / 512)));
+        const int slices    = slicesOf(size, size, fp32 ? 2 : 1);
         const double micros = tileMicros(fp32, size, m, n, k, slices);
-        if (best.size == 0 || micros < least) {
+        if (best.rows == 0 || micros < least) {
             best  = {size, slices};
             least = micros;
         }
@@ -269,12 +275,11 @@ struct Layout {
         const uint64_t row = backward ? tokens * size : pack_w ? padded * size : 1;
         piece = std::min(std::max<uint64_t>(kPieceBytes / std::max<uint64_t>(row, 1) / 256 * 256, 2048), roundUp(classes, 256));
         const int64_t n = backward || pack_w ? std::min<int64_t>(piece, classes) : classes;
-        logits          = tilingOf(p.type, tokens, n, padded, false);
+        logits = tilingOf(p.type, backward ? HeadTile::kGradLogits : HeadTile::kLogSum, tokens, n, padded);
         // Classes of one part: of a 16-bit tile's columns, or of the 64 that an fp32 wave holds.
-        parts      = ceilDiv(classes, p.type == FTRAIN_NUMERIC_TYPE_FP32 ? 64 : logits.size);
-        for_hidden = tilingOf(p.type, tokens, hidden, n, true);
-        // The rows of the weight's gradient are the classes: always many, so fp32 has the large tile only.
-        for_weight = p.type == FTRAIN_NUMERIC_TYPE_FP32 ? Tiling{128, 1} : tilingOf(p.type, n, hidden, tokens, false);
+        parts      = ceilDiv(classes, p.type == FTRAIN_NUMERIC_TYPE_FP32 ? 64 : logits.rows == 256 ? 256 : 128);
+        for_hidden = tilingOf(p.type, HeadTile::kGradHidden, tokens, hidden, n);
+        for_weight = tilingOf(p.type, HeadTile::kGradWeight, n, hidden, tokens);
         slice     = tokens * padded;
         auto take = [&](uint64_t n) {
             const uint64_t at = bytes;
@@ -318,13 +323,13 @@ Buffers packInputs(const CrossEntropy& p, const Layout& l, char* base, bool back
     return b;
 }
 
-void launchHeadTile(FTrainNumericType type, HeadTile what, int size, const HeadTileArgs& args, int slices, hipStream_t stream) {
+void launchHeadTile(FTrainNumericType type, HeadTile what, int rows, const HeadTileArgs& args, int slices, hipStream_t stream) {
     if (type == FTRAIN_NUMERIC_TYPE_FP32)
-        launchHeadTileFp32(what, size, args, slices, stream);
+        launchHeadTileFp32(what, rows, args, slices, stream);
     else if (type == FTRAIN_NUMERIC_TYPE_BF16)
-        launchHeadTileBf16(what, size, args, slices, stream);
+        launchHeadTileBf16(what, rows, args, slices, stream);
     else
-        launchHeadTileFp16(what, size, args, slices, stream);
+        launchHeadTileFp16(what, rows, args, slices, stream);
 }
 
 // The classes from `first` on, `n` of them, in rows of whole 16-byte units.
@@ -355,7 +360,7 @@ void forward(const CrossEntropy& p, char* base, hipStream_t stream) {
     for (int64_t v = 0; v < classes; v += piece) {
         t.n = std::min(piece, classes - v), t.first_class = v;
         t.b = weightPiece<T>(p, l, base, v, t.n, t.ldb, stream);
-        launchHeadTile(p.type, HeadTile::kLogSum, l.logits.size, t, 1, stream);
+        launchHeadTile(p.type, HeadTile::kLogSum, l.logits.rows, t, 1, stream);
     }
     launch(&finishLoss, "cross entropy loss", dim3(static_cast<uint32_t>(ceilDiv(p.hidden.rows, kWave))),
            dim3(kFinishThreads), stream, static_cast<const float2*>(t.part), static_cast<const float*>(t.hit),
@@ -380,7 +385,7 @@ void backward(const CrossEntropy& p, char* base, hipStream_t stream) {
             t.b = w, t.ldb = ldw;
             t.d = base + l.dl, t.ldd = l.piece;
             t.m = tokens, t.n = n, t.k = l.padded;
-            launchHeadTile(p.type, HeadTile::kGradLogits, l.logits.size, t, 1, stream);
+            launchHeadTile(p.type, HeadTile::kGradLogits, l.logits.rows, t, 1, stream);
             t.a = base + l.dl, t.lda = l.piece;
             t.d = base + l.dx, t.ldd = l.padded;
             t.n = l.padded, t.k = n;
@@ -390,14 +395,14 @@ void backward(const CrossEntropy& p, char* base, hipStream_t stream) {
             t.slice          = l.slice;
             t.add            = v > 0;
             const int slices = t.add ? static_cast<int>(ceilDiv(n, t.k_chunk)) : l.for_hidden.slices;
-            launchHeadTile(p.type, HeadTile::kGradHidden, l.for_hidden.size, t, slices, stream);
+            launchHeadTile(p.type, HeadTile::kGradHidden, l.for_hidden.rows, t, slices, stream);
         }
         t.a = base + l.dl, t.lda = l.piece;
         t.b = base + l.x, t.ldb = l.padded;
         t.d = static_cast<T*>(p.grad_weight.data) + v * p.grad_weight.ld, t.ldd = p.grad_weight.ld;
         t.m = n, t.n = hidden, t.k = tokens;
         t.read_m = roundUp(n, unit), t.read_n = l.padded;
-        launchHeadTile(p.type, HeadTile::kGradWeight, l.for_weight.size, t, 1, stream);
+        launchHeadTile(p.type, HeadTile::kGradWeight, l.for_weight.rows, t, 1, stream);
     }
     if (tokens > 0)
         launch(&finishHidden<T>, "cross entropy hidden gradient's rows",

@@ -53,10 +53,11 @@ struct HeadTileArgs {
     bool add;
 };
 
-// Launches the product on tiles of `size` rows and columns; m counts every token, the kernels take the
+// Launches the product on tiles of `rows` rows (16-bit: 256x256, 128x128, 64x128; fp32: 128x128, 64x64;
+// the weight's gradient: not the last of either); m counts every token, the kernels take the
 // packed ones only.
-void launchHeadTileFp32(HeadTile what, int size, const HeadTileArgs& args, int slices, hipStream_t stream);
-void launchHeadTileBf16(HeadTile what, int size, const HeadTileArgs& args, int slices, hipStream_t stream);
-void launchHeadTileFp16(HeadTile what, int size, const HeadTileArgs& args, int slices, hipStream_t stream);
+void launchHeadTileFp32(HeadTile what, int rows, const HeadTileArgs& args, int slices, hipStream_t stream);
+void launchHeadTileBf16(HeadTile what, int rows, const HeadTileArgs& args, int slices, hipStream_t stream);
+void launchHeadTileFp16(HeadTile what, int rows, const HeadTileArgs& args, int slices, hipStream_t stream);
 
 }  // namespace ftrain::train

@@ -3,8 +3,8 @@
 
 namespace ftrain::train {
 
-void launchHeadTileBf16(HeadTile what, int size, const HeadTileArgs& args, int slices, hipStream_t stream) {
-    launchHeadTileHalf<true>(what, size, args, slices, stream);
+void launchHeadTileBf16(HeadTile what, int rows, const HeadTileArgs& args, int slices, hipStream_t stream) {
+    launchHeadTileHalf<true>(what, rows, args, slices, stream);
 }
 
 }  // namespace ftrain::train

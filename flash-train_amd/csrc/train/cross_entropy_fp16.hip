@@ -3,8 +3,8 @@
 
 namespace ftrain::train {
 
-void launchHeadTileFp16(HeadTile what, int size, const HeadTileArgs& args, int slices, hipStream_t stream) {
-    launchHeadTileHalf<false>(what, size, args, slices, stream);
+void launchHeadTileFp16(HeadTile what, int rows, const HeadTileArgs& args, int slices, hipStream_t stream) {
+    launchHeadTileHalf<false>(what, rows, args, slices, stream);
 }
 
 }  // namespace ftrain::train

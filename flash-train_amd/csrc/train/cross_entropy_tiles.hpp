@@ -186,36 +186,42 @@ struct GradLogitsEnd16 {
     }
 };
 
-// ---- 16-bit operands: the 128x128 tile of gemm/dma_tile.hpp.
+// ---- 16-bit operands: the 128x128 and 64x128 tiles of gemm/dma_tile.hpp.
 //
-// Lane (li = lane % 32, h = lane / 32) of wave w holds rows 64 (w / 2) + 32 bi + 8 (r / 4) + 4 h + r % 4,
-// column 64 (w % 2) + 32 bj + li: acc[bi][bj][r].  Both ends turn the tile through LDS (512 bytes a row;
-// the row's halves change places where bit 2 of the row is set, so the two h write to different banks),
-// after which 16 lanes hold 8 adjacent columns each of a row and a wave four rows.
-typedef gemm::ddev::floatx16 TileSums128[2][2];
+// Lane (li = lane % 32, h = lane / 32) of wave w holds rows BM / 2 (w / 2) + 32 bi + 8 (r / 4) + 4 h +
+// r % 4, column 64 (w % 2) + 32 bj + li: acc[bi][bj][r].  Both ends turn the tile through LDS (512 bytes
+// a row; the row's halves change places where bit 2 of the row is set, so the two h write to different
+// banks), after which 16 lanes hold 8 adjacent columns each of a row and a wave four rows.
+template <int BM>
+using TileSums128 = gemm::ddev::floatx16[BM / 64][2];
+// Steps of a wave over its rows.
+template <int BM>
+constexpr int kTurns = BM / 16;
 
-// f(row, column, v[8]) for the 8 steps of every wave, rows and columns within the tile.
-template <class F>
-__device__ __forceinline__ void turned128(TileSums128& acc, char* a, char* b, F&& f) {
+__device__ __forceinline__ int turnedRow(int bm, int t) { return bm / 4 * (threadIdx.x >> 6) + 4 * t + ((threadIdx.x & 63) >> 4); }
+
+// f(t, row, column, v[8]) for the steps t of every wave, rows and columns within the tile.
+template <int BM, class F>
+__device__ __forceinline__ void turned128(TileSums128<BM>& acc, char* a, char* b, F&& f) {
     typedef gemm::ppdev::floatx4 floatx4;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // Rows 0 .. 63, which waves 0 and 1 hold and read again, in a's LDS, the others in b's.
-    char* const lds = wave < 2 ? a : b - 64 * 512;
+    // 64 rows in b's LDS; of 128, rows 0 .. 63, which waves 0 and 1 hold and read again, in a's.
+    char* const lds = BM == 64 ? b : wave < 2 ? a : b - 64 * 512;
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
-    for (int bi = 0; bi < 2; ++bi)
+    for (int bi = 0; bi < BM / 64; ++bi)
 #pragma unroll
         for (int bj = 0; bj < 2; ++bj)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int row = 64 * (wave >> 1) + 32 * bi + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
+                const int row = BM / 2 * (wave >> 1) + 32 * bi + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
                 const int col = 64 * (wave & 1) + 32 * bj + (lane & 31);
                 *reinterpret_cast<float*>(lds + row * 512 + 4 * (col ^ (8 * (row & 4)))) = acc[bi][bj][r];
             }
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
-    for (int t = 0; t < 8; ++t) {
-        const int row = 32 * wave + 4 * t + (lane >> 4), col = 8 * (lane & 15);
+    for (int t = 0; t < kTurns<BM>; ++t) {
+        const int row = turnedRow(BM, t), col = 8 * (lane & 15);
         float v[8];
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
@@ -227,6 +233,7 @@ __device__ __forceinline__ void turned128(TileSums128& acc, char* a, char* b, F&
     }
 }
 
+template <int BM>
 struct LogSumEnd128 {
     const RowInfo* rows;
     float2* part;
@@ -234,12 +241,13 @@ struct LogSumEnd128 {
     int64_t tokens;
     int M, N, first_class;
 
-    __device__ __forceinline__ void operator()(TileSums128& acc, char* a, char* b, int m0, int n0) const {
-        const int rows_left = M - m0, cols_left = N - n0, own = 32 * (threadIdx.x >> 6) + ((threadIdx.x & 63) >> 4);
-        int target[8];
+    __device__ __forceinline__ void operator()(TileSums128<BM>& acc, char* a, char* b, int m0, int n0) const {
+        const int rows_left = M - m0, cols_left = N - n0;
+        int target[kTurns<BM>];
 #pragma unroll
-        for (int t = 0; t < 8; ++t) target[t] = rows[m0 + min(own + 4 * t, rows_left - 1)].target - first_class - n0;
-        turned128(acc, a, b, [&](int t, int row, int col, float (&v)[8]) {
+        for (int t = 0; t < kTurns<BM>; ++t)
+            target[t] = rows[m0 + min(turnedRow(BM, t), rows_left - 1)].target - first_class - n0;
+        turned128<BM>(acc, a, b, [&](int t, int row, int col, float (&v)[8]) {
             float top = -INFINITY, sum = 0.f, x = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -259,7 +267,7 @@ struct LogSumEnd128 {
     }
 };
 
-template <bool BF16>
+template <bool BF16, int BM>
 struct GradLogitsEnd128 {
     using T = std::conditional_t<BF16, bf16, fp16>;
     const RowInfo* rows;
@@ -267,13 +275,13 @@ struct GradLogitsEnd128 {
     int64_t ldd;
     int M, N, padded, first_class;
 
-    __device__ __forceinline__ void operator()(TileSums128& acc, char* a, char* b, int m0, int n0) const {
+    __device__ __forceinline__ void operator()(TileSums128<BM>& acc, char* a, char* b, int m0, int n0) const {
         using gemm::ppdev::pack2;
-        const int rows_left = M - m0, cols_left = N - n0, own = 32 * (threadIdx.x >> 6) + ((threadIdx.x & 63) >> 4);
-        RowInfo info[8];
+        const int rows_left = M - m0, cols_left = N - n0;
+        RowInfo info[kTurns<BM>];
 #pragma unroll
-        for (int t = 0; t < 8; ++t) info[t] = rows[m0 + min(own + 4 * t, rows_left - 1)];
-        turned128(acc, a, b, [&](int t, int row, int col, float (&v)[8]) {
+        for (int t = 0; t < kTurns<BM>; ++t) info[t] = rows[m0 + min(turnedRow(BM, t), rows_left - 1)];
+        turned128<BM>(acc, a, b, [&](int t, int row, int col, float (&v)[8]) {
             const RowInfo r = info[t];
             const int y     = r.target - first_class - n0;
             const float g   = r.target < 0 ? NAN : r.grad;
@@ -408,23 +416,26 @@ __global__ __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_pe
     }
 }
 
-// Three stage buffers: this tile runs where there are few workgroups to a CU (one needs two stages in
-// flight to be busy by itself).
-template <bool BF16, HeadTile WHAT>
-__global__ __launch_bounds__(256, 1) void headTileHalf128(HeadTileArgs h) {
+// BM 128: three stage buffers, as this tile runs where there are few workgroups to a CU (one needs two
+// stages in flight to be busy by itself).  BM 64, for at most 64 tokens, whose products are the weight's
+// reading: @STAGES@
+// ROTATE: neighbouring column tiles start at different stages, or all workgroups would read the same few
+// HBM channels at once where the weight's rows are a power of two apart.
+template <bool BF16, HeadTile WHAT, int BM>
+__global__ __launch_bounds__(256, BM == 64 ? 2 : 1) void headTileHalf128(HeadTileArgs h) {
     using T = std::conditional_t<BF16, bf16, fp16>;
     gemm::HalfGemmParams p{};
-    if (!tileProblem<WHAT>(h, p, 128, 128)) return;
+    if (!tileProblem<WHAT>(h, p, BM, 128)) return;
     p.a = h.a, p.b = h.b, p.d = h.d;
     using gemm::ddev::half_gemm_dma_tile;
     using gemm::ddev::StoreTile;
     if constexpr (WHAT == HeadTile::kLogSum) {
-        using End = LogSumEnd128;
-        half_gemm_dma_tile<BF16, false, true, 128, false, 128, 3, false, End>(
+        using End = LogSumEnd128<BM>;
+        half_gemm_dma_tile<BF16, false, true, 128, false, BM, 3, true, End>(
             p, blockIdx.x, 0, 8, End{h.rows, h.part, h.hit, h.tokens, p.m, p.n, h.first_class});
     } else if constexpr (WHAT == HeadTile::kGradLogits) {
-        using End = GradLogitsEnd128<BF16>;
-        half_gemm_dma_tile<BF16, false, true, 128, false, 128, 3, false, End>(
+        using End = GradLogitsEnd128<BF16, BM>;
+        half_gemm_dma_tile<BF16, false, true, 128, false, BM, 3, true, End>(
             p, blockIdx.x, 0, 8, End{h.rows, static_cast<T*>(h.d), h.ldd, p.m, p.n, (h.n + 7) & ~7, h.first_class});
     } else if constexpr (WHAT == HeadTile::kGradHidden) {
         const int first = blockIdx.z * h.k_chunk;
@@ -433,7 +444,7 @@ __global__ __launch_bounds__(256, 1) void headTileHalf128(HeadTileArgs h) {
         p.k             = max(0, min(h.k_chunk, h.k - first));
         p.d             = static_cast<float*>(h.d) + blockIdx.z * h.slice;
         if (h.add) p.c = p.d;
-        half_gemm_dma_tile<BF16, false, false, 128, false, 128, 3>(p, blockIdx.x);
+        half_gemm_dma_tile<BF16, false, false, 128, false, BM, 3>(p, blockIdx.x);
     } else {
         p.alpha   = h.head->inv_scale;
         p.cd_half = 1;
@@ -476,8 +487,9 @@ __global__ __launch_bounds__(256, 2) void headTileFp32(HeadTileArgs h) {
 }
 
 template <class K>
-void launchHead(K kernel, const char* name, const HeadTileArgs& a, int size, int threads, int slices, hipStream_t stream) {
-    const int64_t tiles = (static_cast<int64_t>(a.m) + size - 1) / size * ((static_cast<int64_t>(a.n) + size - 1) / size);
+void launchHead(K kernel, const char* name, const HeadTileArgs& a, int rows, int cols, int threads, int slices,
+                hipStream_t stream) {
+    const int64_t tiles = (static_cast<int64_t>(a.m) + rows - 1) / rows * ((static_cast<int64_t>(a.n) + cols - 1) / cols);
     if (tiles > INT32_MAX) raise(FTRAIN_STATUS_UNSUPPORTED, "cross entropy: too many tiles (%lld)", (long long)tiles);
     launch(kernel, name, dim3(static_cast<uint32_t>(tiles), 1, static_cast<uint32_t>(slices)), dim3(threads), stream, a);
 }
@@ -486,14 +498,20 @@ constexpr const char* kHeadNames[4] = {"cross entropy logits", "cross entropy lo
                                        "cross entropy weight gradient"};
 
 template <bool BF16>
-void launchHeadTileHalf(HeadTile what, int size, const HeadTileArgs& args, int slices, hipStream_t stream) {
-    constexpr void (*large[4])(HeadTileArgs) = {&headTileHalf<BF16, HeadTile::kLogSum>, &headTileHalf<BF16, HeadTile::kGradLogits>,
-                                                &headTileHalf<BF16, HeadTile::kGradHidden>, &headTileHalf<BF16, HeadTile::kGradWeight>};
-    constexpr void (*small[4])(HeadTileArgs) = {
-        &headTileHalf128<BF16, HeadTile::kLogSum>, &headTileHalf128<BF16, HeadTile::kGradLogits>,
-        &headTileHalf128<BF16, HeadTile::kGradHidden>, &headTileHalf128<BF16, HeadTile::kGradWeight>};
+void launchHeadTileHalf(HeadTile what, int rows, const HeadTileArgs& args, int slices, hipStream_t stream) {
+    using W = HeadTile;
+    constexpr void (*large[4])(HeadTileArgs) = {&headTileHalf<BF16, W::kLogSum>, &headTileHalf<BF16, W::kGradLogits>,
+                                                &headTileHalf<BF16, W::kGradHidden>, &headTileHalf<BF16, W::kGradWeight>};
+    constexpr void (*medium[4])(HeadTileArgs) = {&headTileHalf128<BF16, W::kLogSum, 128>, &headTileHalf128<BF16, W::kGradLogits, 128>,
+                                                 &headTileHalf128<BF16, W::kGradHidden, 128>,
+                                                 &headTileHalf128<BF16, W::kGradWeight, 128>};
+    constexpr void (*small[3])(HeadTileArgs) = {&headTileHalf128<BF16, W::kLogSum, 64>, &headTileHalf128<BF16, W::kGradLogits, 64>,
+                                                &headTileHalf128<BF16, W::kGradHidden, 64>};
     const int i = static_cast<int>(what);
-    launchHead(size == 256 ? large[i] : small[i], kHeadNames[i], args, size, size == 256 ? 512 : 256, slices, stream);
+    if (rows == 256)
+        launchHead(large[i], kHeadNames[i], args, 256, 256, 512, slices, stream);
+    else
+        launchHead(rows == 128 ? medium[i] : small[i], kHeadNames[i], args, rows, 128, 256, slices, stream);
 }
 
 }  // namespace ftrain::train
