@@ -39,6 +39,7 @@ struct PackArgs {
     void* packed;
     int64_t ld, cols, padded;
     int64_t per_block;  // tokens
+    int pair;           // packed rows of each (kFewTokens)
     bool wide, backward, scaled;
 };
 
@@ -122,8 +123,9 @@ __global__ __launch_bounds__(kPackThreads) void packTokens(PackArgs a) {
         __syncthreads();
         for (int64_t i = wave; i < min(last - t0, static_cast<int64_t>(kPackThreads)); i += kWaves)
             if (place[i] >= 0)
-                copyRow(static_cast<const T*>(a.x) + (t0 + i) * a.ld, static_cast<T*>(a.packed) + place[i] * a.padded, a.cols,
-                        a.padded);
+                for (int q = 0; q < a.pair; ++q)
+                    copyRow(static_cast<const T*>(a.x) + (t0 + i) * a.ld,
+                            static_cast<T*>(a.packed) + (static_cast<int64_t>(place[i]) * a.pair + q) * a.padded, a.cols, a.padded);
     }
     if (threadIdx.x == 0 && blockIdx.x == gridDim.x - 1) *a.head = Head{before, scale, 1.f / scale};
 }
@@ -134,6 +136,70 @@ __global__ __launch_bounds__(kThreads) void packWeight(const T* w, int64_t ld, i
     constexpr int kWaves = kThreads / kWave;
     for (int64_t v = static_cast<int64_t>(blockIdx.x) * kWaves + threadIdx.x / kWave; v < rows; v += static_cast<int64_t>(gridDim.x) * kWaves)
         copyRow(w + v * ld, out + v * padded, cols, padded);
+}
+
+// Four adjacent sums, of which `left` lie in the matrix (none: nothing is read), over the slices.
+__device__ __forceinline__ void joinSlices(const float* from, int64_t slice, int slices, int left, float (&v)[4]) {
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (left > 0)
+        for (int z = 0; z < slices; ++z) {
+            const float4 x = *reinterpret_cast<const float4*>(from + z * slice);
+            s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
+        }
+    v[0] = s.x, v[1] = s.y, v[2] = s.z, v[3] = s.w;
+}
+
+// Where k is cut (Tiling), the logits' slices joined, four adjacent classes a lane and a wave 256 of a
+// row: its maximum and sum of exponentials over them, and the target's logit.
+__global__ __launch_bounds__(kThreads) void joinLogSum(const float* logits, int64_t ld, int64_t slice, int slices,
+                                                       const Head* head, const RowInfo* rows, int n, int first_class,
+                                                       int64_t tokens, float2* part, float* hit) {
+    const int64_t row = static_cast<int64_t>(blockIdx.y) * (kThreads / kWave) + threadIdx.x / kWave;
+    const int col     = blockIdx.x * 256 + 4 * (threadIdx.x % kWave);
+    if (row >= head->valid) return;
+    float v[4];
+    joinSlices(logits + row * ld + col, slice, slices, n - col, v);
+    const int at = rows[row].target - first_class - col;
+    float top    = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (col + e >= n) v[e] = -INFINITY;
+        if (e == at && col + e < n) hit[row] = v[e];
+        top = fmaxf(top, v[e]);
+    }
+    top              = groupMax<kWave>(top);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum        = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum += expFast(v[e] - base);
+    sum = groupSum<kWave>(sum);
+    if (threadIdx.x % kWave == 0) part[(first_class / 256 + blockIdx.x) * tokens + row] = make_float2(top, sum);
+}
+
+// The same for dl, with zeros up to `padded` columns.
+template <class T>
+__global__ __launch_bounds__(kThreads) void joinGradLogits(const float* logits, int64_t ld, int64_t slice, int slices,
+                                                           const Head* head, const RowInfo* rows, int n, int padded,
+                                                           int first_class, T* dl, int64_t ldd, int pair) {
+    const int64_t row = static_cast<int64_t>(blockIdx.y) * (kThreads / kWave) + threadIdx.x / kWave;
+    const int col     = blockIdx.x * 256 + 4 * (threadIdx.x % kWave);
+    if (row >= head->valid || col >= padded) return;
+    float v[4];
+    joinSlices(logits + row * ld + col, slice, slices, n - col, v);
+    const RowInfo r = rows[row];
+    const int at    = r.target - first_class - col;
+    const float g   = r.target < 0 ? NAN : r.grad;
+    typedef T vec __attribute__((ext_vector_type(4)));
+    vec out, rest;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float x = col + e < n ? (expFast(v[e] - r.lse) - (e == at ? 1.f : 0.f)) * g : 0.f;
+        out[e]        = static_cast<T>(x);
+        rest[e]       = static_cast<T>(x - toFloat(static_cast<T>(x)));
+    }
+    T* const to                 = dl + row * pair * ldd + col;
+    *reinterpret_cast<vec*>(to) = out;
+    if (pair == 2) *reinterpret_cast<vec*>(to + ldd) = rest;
 }
 
 // loss and lse of every kept token from its parts' maxima and sums: lanes take adjacent tokens, the
@@ -181,18 +247,19 @@ __global__ __launch_bounds__(kFinishThreads) void finishLoss(const float2* part,
 template <class T>
 __global__ __launch_bounds__(kThreads) void finishHidden(const float* sums, int64_t ld, const int32_t* place,
                                                          const Head* head, T* out, int64_t out_ld, int64_t tokens,
-                                                         int64_t cols, int slices, int64_t slice) {
+                                                         int64_t cols, int slices, int64_t slice, int pair) {
     const float inv = head->inv_scale;
     for (int64_t t = blockIdx.x; t < tokens; t += gridDim.x) {
         const int row           = place[t];
-        const float* const from = sums + static_cast<int64_t>(row) * ld;
+        const float* const from = sums + static_cast<int64_t>(row) * pair * ld;
         for (int64_t i = threadIdx.x * 4; i < cols; i += kThreads * 4) {
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
             if (row >= 0) {
-                for (int z = 0; z < slices; ++z) {
-                    const float4 x = *reinterpret_cast<const float4*>(from + z * slice + i);
-                    v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
-                }
+                for (int z = 0; z < slices; ++z)
+                    for (int q = 0; q < pair; ++q) {
+                        const float4 x = *reinterpret_cast<const float4*>(from + z * slice + q * ld + i);
+                        v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+                    }
             }
             T* const to = out + t * out_ld + i;
             to[0]       = static_cast<T>(v.x * inv);
@@ -217,41 +284,59 @@ struct Tiling {
 };
 
 // Modelled time of an m x n x k product, us: rounds of the 256 CUs, each of its stages and a start and
-// end.  Measured per stage: 16-bit (64 k) 256x256 1.25 (0.75 with at most 128 rows), 128x128 0.5; fp32
-// (32 k) 128x128 1.75, 64x64 0.5.  A large tile reads less for each product, a small one fills the CUs
+// end.  Measured per stage: 16-bit (64 k) 256x256 1.25 (0.75 with at most 128 rows), 128x128 0.5, 64x128 0.3;
+// fp32 (32 k) 128x128 1.75, 64x64 0.5.  A large tile reads less for each product, a small one fills the CUs
 // where there are few:
 //   bf16, us, 256x256 / 128x128: loss of 128 x 1024 x 8192 27.8 / 24.0, 500 x 1024 x 5003 40.5 / 23.2,
 //     64 x 4096 x 128000 201 / 234; gradients of 500 x 1024 x 5003 77.6 / 60.2, 2048 x 4096 x 32003
 //     1198 / 1392;
 //   fp32, us, 128x128 / 64x64: loss of 300 x 8192 x 3000 470 / 166, 1000 x 1000 x 1000 80 / 36.
-double tileMicros(bool fp32, int size, int64_t m, int64_t n, int64_t k, int slices) {
-    const double stage = fp32 ? (size == 128 ? 1.75 : 0.5) : size == 256 ? (m <= 128 ? 0.75 : 1.25) : 0.5;
-    const double ends  = fp32 ? 5.0 : size == 256 ? 9.0 : 6.0;
-    const uint64_t rounds = ceilDiv(ceilDiv(m, size) * ceilDiv(n, size) * slices, kCus);
+double tileMicros(bool fp32, int rows, int cols, int64_t m, int64_t n, int64_t k, int slices) {
+    const double stage = fp32 ? (rows == 128 ? 1.75 : 0.5) : rows == 256 ? (m <= 128 ? 0.75 : 1.25) : rows == 128 ? 0.5 : 0.3;
+    const double ends  = fp32 ? 5.0 : rows == 256 ? 9.0 : 6.0;
+    const uint64_t rounds = ceilDiv(ceilDiv(m, rows) * ceilDiv(n, cols) * slices, kCus);
     return static_cast<double>(rounds) * (static_cast<double>(ceilDiv(k, slices)) / (fp32 ? 32 : 64) * stage + ends);
 }
 
-// sliced: k may be cut until the tiles fill the device (two workgroups of fp32 and of the 64x128 tile run
-// on a CU), in slices of at least 512.
+// Most bytes of the logits' slices, and what a further launch to join them takes, us.
+constexpr uint64_t kSliceBytes = 64ull << 20;
+constexpr double kJoinMicros   = 5.0;
+
+// k may be cut, in slices of at least 512, until the tiles fill the device (two workgroups of fp32 and of
+// the 64x128 tile run on a CU): dx's always, as its sums are fp32 in the workspace anyway; the logits'
+// where few tokens' few tiles have a long k, at the price of writing and reading the slices (at 4 TB/s)
+// and a launch: gradients of 16 x 8192 x 4000 fp32 255 -> 146 us.  (With 200 x 4096 x 10000 8% of
+// 528 us: not done.)
 Tiling tilingOf(FTrainNumericType type, HeadTile what, int64_t m, int64_t n, int64_t k) {
-    const bool fp32 = type == FTRAIN_NUMERIC_TYPE_FP32, sliced = what == HeadTile::kGradHidden;
-    auto slicesOf = [&](int rows, int cols, int at_once) {
-        const uint64_t tiles = std::max<uint64_t>(1, ceilDiv(m, rows) * ceilDiv(n, cols));
-        return sliced ? static_cast<int>(std::max<uint64_t>(1, std::min<uint64_t>(at_once * kCus / tiles, k / 512))) : 1;
-    };
+    const bool fp32 = type == FTRAIN_NUMERIC_TYPE_FP32, hidden = what == HeadTile::kGradHidden;
     // The rows of the weight's gradient are the classes: many, and fp32 has the large tile only.
     if (fp32 && what == HeadTile::kGradWeight) return {128, 1};
-    // At most 64 tokens: 16x4096x32003 bf16 loss @FEW@.
-    if (!fp32 && what != HeadTile::kGradWeight && m <= 64) return {64, slicesOf(64, 128, 2)};
     Tiling best{};
     double least = 0.0;
-    for (const int size : {fp32 ? 128 : 256, fp32 ? 64 : 128}) {
-        const int slices    = slicesOf(size, size, fp32 ? 2 : 1);
-        const double micros = tileMicros(fp32, size, m, n, k, slices);
-        if (best.rows == 0 || micros < least) {
-            best  = {size, slices};
-            least = micros;
+    auto consider = [&](int rows, int cols, int at_once) {
+        const uint64_t tiles = std::max<uint64_t>(1, ceilDiv(m, rows) * ceilDiv(n, cols));
+        const int most       = static_cast<int>(std::max<uint64_t>(1, std::min<uint64_t>(at_once * kCus / tiles, k / 512)));
+        auto offer           = [&](int slices, double more) {
+            const double micros = tileMicros(fp32, rows, cols, m, n, k, slices) + more;
+            if (best.rows == 0 || micros < least) {
+                best  = {rows, slices};
+                least = micros;
+            }
+        };
+        if (hidden) {
+            offer(most, 0.0);
+            return;
         }
+        offer(1, 0.0);
+        const double bytes = 4.0 * m * roundUp(n, 256) * most;
+        if (what != HeadTile::kGradWeight && m <= kFewTokens && most > 1 && bytes <= kSliceBytes)
+            offer(most, kJoinMicros + 2.0 * bytes / 4e6);
+    };
+    if (!fp32 && what != HeadTile::kGradWeight && m <= kFewTokens) {
+        consider(64, 128, 2);
+    } else {
+        consider(fp32 ? 128 : 256, fp32 ? 128 : 256, fp32 ? 2 : 1);
+        consider(fp32 ? 64 : 128, fp32 ? 64 : 128, fp32 ? 2 : 1);
     }
     return best;
 }
@@ -259,28 +344,35 @@ Tiling tilingOf(FTrainNumericType type, HeadTile what, int64_t m, int64_t n, int
 // The workspace, laid out for one call.
 struct Layout {
     uint64_t bytes = 0;
-    uint64_t head, place, rows, x, w, part, hit, dl, dx;
+    uint64_t head, place, rows, x, w, part, hit, cut, dl, dx;
     int64_t padded;  // columns of a packed row of x (and w)
     int64_t piece;   // classes of one piece
+    int64_t pair;    // rows of x and dl of each token (kFewTokens)
     int64_t parts;
     Tiling logits, for_hidden, for_weight;
+    int64_t cut_ld;  // row stride of the logits' slices, where k is cut
     int64_t slice;   // elements of one slice's sums
     bool pack_w;     // the weight's rows are not whole 16-byte units: each piece is copied first
 
     Layout(const CrossEntropy& p, bool backward) {
         const uint64_t tokens = p.hidden.rows, hidden = p.hidden.cols, classes = p.weight.rows;
         const uint64_t size = elementBytes(p.type), unit = 16 / size;
+        pair   = backward && size == 2 && tokens <= kFewTokens ? 2 : 1;
         padded = roundUp(hidden, unit);
         pack_w = hidden % unit != 0 || p.weight.ld % unit != 0 || reinterpret_cast<uintptr_t>(p.weight.data) % 16 != 0;
-        const uint64_t row = backward ? tokens * size : pack_w ? padded * size : 1;
+        const uint64_t row = backward ? pair * tokens * size : pack_w ? padded * size : 1;
         piece = std::min(std::max<uint64_t>(kPieceBytes / std::max<uint64_t>(row, 1) / 256 * 256, 2048), roundUp(classes, 256));
         const int64_t n = backward || pack_w ? std::min<int64_t>(piece, classes) : classes;
         logits = tilingOf(p.type, backward ? HeadTile::kGradLogits : HeadTile::kLogSum, tokens, n, padded);
-        // Classes of one part: of a 16-bit tile's columns, or of the 64 that an fp32 wave holds.
-        parts      = ceilDiv(classes, p.type == FTRAIN_NUMERIC_TYPE_FP32 ? 64 : logits.rows == 256 ? 256 : 128);
-        for_hidden = tilingOf(p.type, HeadTile::kGradHidden, tokens, hidden, n);
-        for_weight = tilingOf(p.type, HeadTile::kGradWeight, n, hidden, tokens);
-        slice     = tokens * padded;
+        // Classes of one part: a 16-bit tile's columns, the 64 that an fp32 wave holds, or joinLogSum's.
+        parts      = ceilDiv(classes, logits.slices > 1               ? 256
+                                      : p.type == FTRAIN_NUMERIC_TYPE_FP32 ? 64
+                                      : logits.rows == 256                 ? 256
+                                                                           : 128);
+        cut_ld     = roundUp(n, 256);
+        for_hidden = tilingOf(p.type, HeadTile::kGradHidden, pair * tokens, hidden, n);
+        for_weight = tilingOf(p.type, HeadTile::kGradWeight, n, hidden, pair * tokens);
+        slice     = pair * tokens * padded;
         auto take = [&](uint64_t n) {
             const uint64_t at = bytes;
             bytes += roundUp(n, 256);
@@ -289,11 +381,12 @@ struct Layout {
         head  = take(sizeof(Head));
         place = take(tokens * 4);
         rows  = take(tokens * sizeof(RowInfo));
-        x     = take(tokens * padded * size);
+        x     = take(pair * tokens * padded * size);
         w     = pack_w ? take(piece * padded * size) : 0;
         part  = backward ? 0 : take(tokens * parts * sizeof(float2));
         hit   = backward ? 0 : take(tokens * 4);
-        dl    = backward ? take(tokens * piece * size) : 0;
+        cut   = logits.slices > 1 ? take(logits.slices * tokens * cut_ld * 4) : 0;
+        dl    = backward ? take(pair * tokens * piece * size) : 0;
         dx    = backward ? take(for_hidden.slices * slice * 4) : 0;
     }
 };
@@ -315,7 +408,7 @@ Buffers packInputs(const CrossEntropy& p, const Layout& l, char* base, bool back
     a.loss = p.loss, a.lse = p.lse, a.grad_loss = p.grad_loss;
     a.head = b.head, a.place = b.place, a.rows = b.rows;
     a.x = p.hidden.data, a.ld = p.hidden.ld, a.cols = p.hidden.cols;
-    a.packed = base + l.x, a.padded = l.padded;
+    a.packed = base + l.x, a.padded = l.padded, a.pair = static_cast<int>(l.pair);
     a.backward = backward, a.scaled = backward && p.type == FTRAIN_NUMERIC_TYPE_FP16;
     a.per_block        = std::max<int64_t>(1, ceilDiv(a.tokens, kPackBlocks));
     const int64_t grid = std::max<int64_t>(1, ceilDiv(a.tokens, a.per_block));
@@ -346,6 +439,16 @@ const T* weightPiece(const CrossEntropy& p, const Layout& l, char* base, int64_t
     return to;
 }
 
+// The logits' slices of the classes that t describes.
+void cutLogits(const CrossEntropy& p, const Layout& l, char* base, HeadTileArgs t, hipStream_t stream) {
+    t.d = base + l.cut, t.ldd = l.cut_ld, t.slice = p.hidden.rows * l.cut_ld;
+    t.k_chunk = roundUp(ceilDiv(t.k, l.logits.slices), 64);
+    launchHeadTile(p.type, HeadTile::kLogits, l.logits.rows, t, l.logits.slices, stream);
+}
+dim3 joinGrid(int64_t tokens, int64_t n) {
+    return dim3(static_cast<uint32_t>(ceilDiv(n, 256)), static_cast<uint32_t>(ceilDiv(tokens, kThreads / kWave)));
+}
+
 template <class T>
 void forward(const CrossEntropy& p, char* base, hipStream_t stream) {
     const Layout l(p, false);
@@ -360,7 +463,14 @@ void forward(const CrossEntropy& p, char* base, hipStream_t stream) {
     for (int64_t v = 0; v < classes; v += piece) {
         t.n = std::min(piece, classes - v), t.first_class = v;
         t.b = weightPiece<T>(p, l, base, v, t.n, t.ldb, stream);
-        launchHeadTile(p.type, HeadTile::kLogSum, l.logits.rows, t, 1, stream);
+        if (l.logits.slices == 1) {
+            launchHeadTile(p.type, HeadTile::kLogSum, l.logits.rows, t, 1, stream);
+            continue;
+        }
+        cutLogits(p, l, base, t, stream);
+        launch(&joinLogSum, "cross entropy join", joinGrid(t.m, t.n), dim3(kThreads), stream,
+               reinterpret_cast<const float*>(base + l.cut), l.cut_ld, t.m * l.cut_ld, l.logits.slices,
+               static_cast<const Head*>(b.head), static_cast<const RowInfo*>(b.rows), t.n, t.first_class, t.tokens, t.part, t.hit);
     }
     launch(&finishLoss, "cross entropy loss", dim3(static_cast<uint32_t>(ceilDiv(p.hidden.rows, kWave))),
            dim3(kFinishThreads), stream, static_cast<const float2*>(t.part), static_cast<const float*>(t.hit),
@@ -376,19 +486,28 @@ void backward(const CrossEntropy& p, char* base, hipStream_t stream) {
     const int64_t unit = 16 / sizeof(T);
     for (int64_t v = 0; v < classes; v += l.piece) {
         HeadTileArgs t{};
-        t.head = b.head, t.rows = b.rows, t.first_class = v;
+        t.head = b.head, t.rows = b.rows, t.first_class = v, t.pair = static_cast<int32_t>(l.pair);
         const int64_t n = std::min(l.piece, classes - v);
         int64_t ldw;
         const T* const w = weightPiece<T>(p, l, base, v, n, ldw, stream);
         if (tokens > 0) {
-            t.a = base + l.x, t.lda = l.padded;
+            t.a = base + l.x, t.lda = l.pair * l.padded;
             t.b = w, t.ldb = ldw;
             t.d = base + l.dl, t.ldd = l.piece;
             t.m = tokens, t.n = n, t.k = l.padded;
-            launchHeadTile(p.type, HeadTile::kGradLogits, l.logits.rows, t, 1, stream);
+            if (l.logits.slices == 1) {
+                launchHeadTile(p.type, HeadTile::kGradLogits, l.logits.rows, t, 1, stream);
+            } else {
+                cutLogits(p, l, base, t, stream);
+                launch(&joinGradLogits<T>, "cross entropy join", joinGrid(tokens, n), dim3(kThreads), stream,
+                       reinterpret_cast<const float*>(base + l.cut), l.cut_ld, tokens * l.cut_ld, l.logits.slices,
+                       static_cast<const Head*>(b.head), static_cast<const RowInfo*>(b.rows), t.n,
+                       static_cast<int>(roundUp(n, unit)), t.first_class, reinterpret_cast<T*>(base + l.dl), l.piece,
+                       static_cast<int>(l.pair));
+            }
             t.a = base + l.dl, t.lda = l.piece;
             t.d = base + l.dx, t.ldd = l.padded;
-            t.n = l.padded, t.k = n;
+            t.m = l.pair * tokens, t.n = l.padded, t.k = n;
             // Whole stages of the tile to a slice; a last piece's slices may be fewer, its sums then
             // leave the others as they are.
             t.k_chunk        = roundUp(ceilDiv(n, l.for_hidden.slices), 64);
@@ -400,7 +519,7 @@ void backward(const CrossEntropy& p, char* base, hipStream_t stream) {
         t.a = base + l.dl, t.lda = l.piece;
         t.b = base + l.x, t.ldb = l.padded;
         t.d = static_cast<T*>(p.grad_weight.data) + v * p.grad_weight.ld, t.ldd = p.grad_weight.ld;
-        t.m = n, t.n = hidden, t.k = tokens;
+        t.m = n, t.n = hidden, t.k = l.pair * tokens;
         t.read_m = roundUp(n, unit), t.read_n = l.padded;
         launchHeadTile(p.type, HeadTile::kGradWeight, l.for_weight.rows, t, 1, stream);
     }
@@ -409,7 +528,7 @@ void backward(const CrossEntropy& p, char* base, hipStream_t stream) {
                dim3(static_cast<uint32_t>(std::min<int64_t>(tokens, 65536))), dim3(kThreads), stream,
                reinterpret_cast<const float*>(base + l.dx), l.padded, static_cast<const int32_t*>(b.place),
                static_cast<const Head*>(b.head), static_cast<T*>(p.grad_hidden.data), p.grad_hidden.ld, tokens, hidden,
-               l.for_hidden.slices, l.slice);
+               l.for_hidden.slices, l.slice, static_cast<int>(l.pair));
 }
 
 }  // namespace

@@ -30,7 +30,15 @@ enum class HeadTile {
     kGradLogits,  // tokens x classes: dl
     kGradHidden,  // tokens x hidden = dl w, fp32 sums of a slice of the classes
     kGradWeight,  // classes x hidden = dl^T x
+    kLogits,      // tokens x classes: fp32 sums of a slice of the hidden values
 };
+
+// Up to this many tokens (16-bit types) the products are the weight's reading, and the arithmetic is free:
+// the smallest tile's rows, k of the logits cut where the tiles are few, and dl kept in two adjacent rows,
+// its value rounded and what that left (twice the mantissa), against two equal rows of x.  With one
+// rounding the gradients of 16 tokens, where single values of dl count, were 1.6 times as far from 64 bits
+// as the rounding of the result alone; of many tokens 1.4 times.
+constexpr int64_t kFewTokens = 64;
 
 struct HeadTileArgs {
     const void *a, *b;
@@ -40,21 +48,22 @@ struct HeadTileArgs {
     int32_t read_m, read_n;  // what the storage of transposed operands holds; 0: m, n
     const Head* head;
     const RowInfo* rows;
+    int32_t pair;  // kGradHidden, kGradWeight: rows of dl (and x) of each packed token (kFewTokens)
     int32_t first_class;
     // kLogSum: a pair of maximum and sum of each part of the classes and, within it, of each of `tokens`
     // rows; the logit of each row's target.
     float2* part;
     float* hit;
     int64_t tokens;
-    // kGradHidden: the classes of one of gridDim.z slices, elements from one slice's sums to the next's,
-    // and whether the sums of earlier classes are added to.
+    // kGradHidden, kLogits: the k of one of gridDim.z slices, elements from one slice's sums to the next's,
+    // and (kGradHidden) whether the sums of earlier classes are added to.
     int32_t k_chunk;
     int64_t slice;
     bool add;
 };
 
 // Launches the product on tiles of `rows` rows (16-bit: 256x256, 128x128, 64x128; fp32: 128x128, 64x64;
-// the weight's gradient: not the last of either); m counts every token, the kernels take the
+// the weight's gradient: not the last of either; kLogits: not 256x256); m counts every token, the kernels take the
 // packed ones only.
 void launchHeadTileFp32(HeadTile what, int rows, const HeadTileArgs& args, int slices, hipStream_t stream);
 void launchHeadTileBf16(HeadTile what, int rows, const HeadTileArgs& args, int slices, hipStream_t stream);

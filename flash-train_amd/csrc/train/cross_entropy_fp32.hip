@@ -4,10 +4,12 @@
 namespace ftrain::train {
 
 void launchHeadTileFp32(HeadTile what, int rows, const HeadTileArgs& args, int slices, hipStream_t stream) {
-    constexpr void (*large[4])(HeadTileArgs) = {&headTileFp32<HeadTile::kLogSum, 128>, &headTileFp32<HeadTile::kGradLogits, 128>,
-                                                &headTileFp32<HeadTile::kGradHidden, 128>, &headTileFp32<HeadTile::kGradWeight, 128>};
-    constexpr void (*small[3])(HeadTileArgs) = {&headTileFp32<HeadTile::kLogSum, 64>, &headTileFp32<HeadTile::kGradLogits, 64>,
-                                                &headTileFp32<HeadTile::kGradHidden, 64>};
+    using W = HeadTile;
+    constexpr void (*large[5])(HeadTileArgs) = {&headTileFp32<W::kLogSum, 128>, &headTileFp32<W::kGradLogits, 128>,
+                                                &headTileFp32<W::kGradHidden, 128>, &headTileFp32<W::kGradWeight, 128>,
+                                                &headTileFp32<W::kLogits, 128>};
+    constexpr void (*small[5])(HeadTileArgs) = {&headTileFp32<W::kLogSum, 64>, &headTileFp32<W::kGradLogits, 64>,
+                                                &headTileFp32<W::kGradHidden, 64>, nullptr, &headTileFp32<W::kLogits, 64>};
     const int i = static_cast<int>(what);
     launchHead(rows == 128 ? large[i] : small[i], kHeadNames[i], args, rows, rows, 256, slices, stream);
 }

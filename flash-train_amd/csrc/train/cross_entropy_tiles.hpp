@@ -290,9 +290,20 @@ struct GradLogitsEnd128 {
                 v[e] = (expFast(v[e] - r.lse) - (col + e == y ? 1.f : 0.f)) * g;
                 if (col + e >= cols_left) v[e] = 0.f;
             }
-            if (row < rows_left && n0 + col < padded)
-                *reinterpret_cast<gemm::ppdev::u32x4*>(d + (m0 + row) * ldd + n0 + col) = gemm::ppdev::u32x4{
+            if (row >= rows_left || n0 + col >= padded) return;
+            // Two rows a token on the 64-row tile (kFewTokens).
+            constexpr int kPair = BM == 64 ? 2 : 1;
+            T* const to         = d + (m0 + row) * kPair * ldd + n0 + col;
+            auto store          = [&](T* at) {
+                *reinterpret_cast<gemm::ppdev::u32x4*>(at) = gemm::ppdev::u32x4{
                     pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]), pack2<BF16>(v[4], v[5]), pack2<BF16>(v[6], v[7])};
+            };
+            store(to);
+            if constexpr (kPair == 2) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] -= toFloat(static_cast<T>(v[e]));
+                store(to + ldd);
+            }
         });
     }
 };
@@ -372,7 +383,7 @@ struct GradWeightEnd {
 // packed than tokens).
 template <HeadTile WHAT, class P>
 __device__ __forceinline__ bool tileProblem(const HeadTileArgs& h, P& p, int size, int tile_cols) {
-    const int valid = h.head->valid;
+    const int valid = h.head->valid * (WHAT == HeadTile::kGradHidden || WHAT == HeadTile::kGradWeight ? h.pair : 1);
     p.m = h.m, p.n = h.n, p.k = h.k;
     p.lda = h.lda, p.ldb = h.ldb, p.ldd = p.ldc = h.ldd;
     p.alpha = p.beta = 1.f;
@@ -445,6 +456,13 @@ __global__ __launch_bounds__(256, BM == 64 ? 2 : 1) void headTileHalf128(HeadTil
         p.d             = static_cast<float*>(h.d) + blockIdx.z * h.slice;
         if (h.add) p.c = p.d;
         half_gemm_dma_tile<BF16, false, false, 128, false, BM, 3>(p, blockIdx.x);
+    } else if constexpr (WHAT == HeadTile::kLogits) {
+        const int first = blockIdx.z * h.k_chunk;
+        p.a             = static_cast<const T*>(h.a) + first;
+        p.b             = static_cast<const T*>(h.b) + first;
+        p.k             = max(0, min(h.k_chunk, h.k - first));
+        p.d             = static_cast<float*>(h.d) + blockIdx.z * h.slice;
+        half_gemm_dma_tile<BF16, false, true, 128, false, BM, 3, true>(p, blockIdx.x);
     } else {
         p.alpha   = h.head->inv_scale;
         p.cd_half = 1;
@@ -452,12 +470,12 @@ __global__ __launch_bounds__(256, BM == 64 ? 2 : 1) void headTileHalf128(HeadTil
     }
 }
 
-// FOLD 16: sums of 512 k.  An fp32 sum of all of k = 2048 .. 8192 in one chain left dl off by 6e-6 to
-// 1.5e-5 of its size (a logit of 16 is off by half a unit of 2^-20 at every step); folded, by 1.5e-6.  It
-// costs 5% on 2048 x 2048 x 32003 (5221 -> 5486 us for the gradients).
+// Sums of k in one chain, as in the GEMM itself: dl's error is that of an fp32 product's logits (5e-6 of
+// its size at k = 2048, 1.5e-5 at 8192).  Sums of 512 k added up apart took a third to a tenth of that
+// error and 5% more time (16 accumulators' worth of spills at 256 registers).
 template <HeadTile WHAT, int BM>
 __global__ __launch_bounds__(256, 2) void headTileFp32(HeadTileArgs h) {
-    constexpr int WM = BM == 128 ? 2 : 4, WN = BM == 128 ? 2 : 1, kFold = 16;
+    constexpr int WM = BM == 128 ? 2 : 4, WN = BM == 128 ? 2 : 1;
     gemm::GemmParams p{};
     if (!tileProblem<WHAT>(h, p, BM, BM)) return;
     p.a = static_cast<const float*>(h.a), p.b = static_cast<const float*>(h.b), p.d = static_cast<float*>(h.d);
@@ -465,11 +483,11 @@ __global__ __launch_bounds__(256, 2) void headTileFp32(HeadTileArgs h) {
     using gemm::d32::StoreTile;
     if constexpr (WHAT == HeadTile::kLogSum) {
         using End = LogSumEnd32;
-        fp32_gemm_dma_tile<BM, BM, WM, WN, false, true, false, false, End, kFold>(
+        fp32_gemm_dma_tile<BM, BM, WM, WN, false, true, false, false, End>(
             p, blockIdx.x, 0, 4, End{h.rows, h.part, h.hit, h.tokens, h.first_class});
     } else if constexpr (WHAT == HeadTile::kGradLogits) {
         using End = GradLogitsEnd32;
-        fp32_gemm_dma_tile<BM, BM, WM, WN, false, true, false, false, End, kFold>(
+        fp32_gemm_dma_tile<BM, BM, WM, WN, false, true, false, false, End>(
             p, blockIdx.x, 0, 4, End{h.rows, static_cast<float*>(h.d), h.ldd, (h.n + 3) & ~3, h.first_class});
     } else if constexpr (WHAT == HeadTile::kGradHidden) {
         const int first = blockIdx.z * h.k_chunk;
@@ -478,10 +496,19 @@ __global__ __launch_bounds__(256, 2) void headTileFp32(HeadTileArgs h) {
         p.k = max(0, min(h.k_chunk, h.k - first));
         p.d += blockIdx.z * h.slice;
         if (h.add) p.c = p.d;
-        fp32_gemm_dma_tile<BM, BM, WM, WN, false, false, false, false, StoreTile, kFold>(p, blockIdx.x, 0);
+        fp32_gemm_dma_tile<BM, BM, WM, WN, false, false, false, false, StoreTile>(p, blockIdx.x, 0);
+    } else if constexpr (WHAT == HeadTile::kLogits) {
+        const int first = blockIdx.z * h.k_chunk;
+        p.a += first;
+        p.b += first;
+        p.k = max(0, min(h.k_chunk, h.k - first));
+        p.d += blockIdx.z * h.slice;
+        // Whole chunks of four columns are stored; the row stride has room for them.
+        p.n = (h.n + 3) & ~3;
+        fp32_gemm_dma_tile<BM, BM, WM, WN, false, true, false, false, StoreTile>(p, blockIdx.x, 0, 4, StoreTile{}, 0, h.n);
     } else {
         using End = GradWeightEnd;
-        fp32_gemm_dma_tile<BM, BM, WM, WN, false, false, true, false, End, kFold>(
+        fp32_gemm_dma_tile<BM, BM, WM, WN, false, false, true, false, End>(
             p, blockIdx.x, 0, 4, End{static_cast<float*>(h.d), h.ldd}, h.read_m, h.read_n);
     }
 }
@@ -494,19 +521,20 @@ void launchHead(K kernel, const char* name, const HeadTileArgs& a, int rows, int
     launch(kernel, name, dim3(static_cast<uint32_t>(tiles), 1, static_cast<uint32_t>(slices)), dim3(threads), stream, a);
 }
 
-constexpr const char* kHeadNames[4] = {"cross entropy logits", "cross entropy logits' gradient", "cross entropy hidden gradient",
-                                       "cross entropy weight gradient"};
+constexpr const char* kHeadNames[5] = {"cross entropy loss", "cross entropy logits' gradient", "cross entropy hidden gradient",
+                                       "cross entropy weight gradient", "cross entropy logits"};
 
 template <bool BF16>
 void launchHeadTileHalf(HeadTile what, int rows, const HeadTileArgs& args, int slices, hipStream_t stream) {
     using W = HeadTile;
     constexpr void (*large[4])(HeadTileArgs) = {&headTileHalf<BF16, W::kLogSum>, &headTileHalf<BF16, W::kGradLogits>,
                                                 &headTileHalf<BF16, W::kGradHidden>, &headTileHalf<BF16, W::kGradWeight>};
-    constexpr void (*medium[4])(HeadTileArgs) = {&headTileHalf128<BF16, W::kLogSum, 128>, &headTileHalf128<BF16, W::kGradLogits, 128>,
-                                                 &headTileHalf128<BF16, W::kGradHidden, 128>,
-                                                 &headTileHalf128<BF16, W::kGradWeight, 128>};
-    constexpr void (*small[3])(HeadTileArgs) = {&headTileHalf128<BF16, W::kLogSum, 64>, &headTileHalf128<BF16, W::kGradLogits, 64>,
-                                                &headTileHalf128<BF16, W::kGradHidden, 64>};
+    constexpr void (*medium[5])(HeadTileArgs) = {
+        &headTileHalf128<BF16, W::kLogSum, 128>, &headTileHalf128<BF16, W::kGradLogits, 128>, &headTileHalf128<BF16, W::kGradHidden, 128>,
+        &headTileHalf128<BF16, W::kGradWeight, 128>, &headTileHalf128<BF16, W::kLogits, 128>};
+    constexpr void (*small[5])(HeadTileArgs) = {&headTileHalf128<BF16, W::kLogSum, 64>, &headTileHalf128<BF16, W::kGradLogits, 64>,
+                                                &headTileHalf128<BF16, W::kGradHidden, 64>, nullptr,
+                                                &headTileHalf128<BF16, W::kLogits, 64>};
     const int i = static_cast<int>(what);
     if (rows == 256)
         launchHead(large[i], kHeadNames[i], args, 256, 256, 512, slices, stream);
