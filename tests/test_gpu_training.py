@@ -208,6 +208,29 @@ def test_cross_entropy_reductions(ft):
         ft.linear_cross_entropy(a, b, y.cuda(), reduction="median")
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(16, 2048, 300), (1, 4096, 50), (64, 1500, 700), (33, 1100, 129), (65, 1024, 1000),
+                                   (300, 136, 40001), (500, 40, 30000), (1000, 700, 256)])
+def test_cross_entropy_on_every_tile(ft, shape, dtype):
+    """Few tokens with a long sum (cut across workgroups), and products large enough for the large tiles."""
+    check_head(ft, *head(*shape, dtype, ignored=0.1 if shape[0] > 1 else 0.0, seed=20))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hidden", [64, 59])
+def test_cross_entropy_in_several_pieces(ft, hidden, dtype):
+    """dl of 8192 tokens in pieces of 16384 (16-bit) or 8192 classes; 59: the weight's rows are packed too."""
+    x, w, y, grad = head(8192, hidden, 40003, dtype, ignored=0.1, seed=23)
+    dev = [t.cuda() for t in (x, w, y, grad)]
+    loss, lse = ft.linear_cross_entropy_forward(*dev[:3])
+    exact, exact_lse, bound = cross_entropy(*dev[:3])
+    assert ((loss.double() - exact).abs() <= bound).all() and ((lse.double() - exact_lse).abs() <= bound).all()
+    saved = exact_lse.float()
+    gx, gw = ft.linear_cross_entropy_backward(dev[3], *dev[:3], saved)
+    ex, ew, bx, bw = cross_entropy_grads(dev[3], *dev[:3], saved)
+    assert ((gx.double() - ex).abs() <= bx).all() and ((gw.double() - ew).abs() <= bw).all()
+
+
 def test_cross_entropy_past_32_bit_offsets(ft):
     """A weight of more than 2^32 bytes; classes at both ends of it."""
     tokens, hidden, classes = 6, 8192, 270001
@@ -485,6 +508,48 @@ def test_training_operators_in_a_graph(ft):
         torch.cuda.synchronize()
         want = step(ft, fresh)
         assert all(torch.equal(a, b) for a, b in zip(got, want)), seed
+
+
+def test_training_operators_in_the_example_step(ft):
+    """The example's step (router, grouped products, head, clipping) learns its batch, and its gradients
+    are those of the same model written with torch's operators in fp32."""
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "moe_training_step.py")
+    spec = importlib.util.spec_from_file_location("moe_training_step", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    losses = example.train(12, 512, 128, 1003)
+    assert all(math.isfinite(v) for v in losses) and losses[-1] < 0.7 * losses[0], losses
+
+    model = example.Model(64, 307, 6, 2, seed=3)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    batch = torch.randint(0, 307, (200,), generator=g, device="cuda")
+    mask = torch.rand(200, generator=g, device="cuda") < 0.8
+    target = torch.where(mask, (batch + 1) % 307, IGNORE)
+    loss = model.loss(batch, target, mask)
+    loss.backward()
+    # The same choices: the router's logits are computed in bf16 in both.
+    r = ft.moe_route((model.embedding[batch] @ model.router.t()).detach(), 2, True, mask)
+    plain = [p.detach().float().requires_grad_() for p in model.parameters()]
+    emb, router, up, down, out = plain
+    x = emb[batch]
+    p = torch.softmax(x @ router.t(), 1)
+    y = x
+    for k in range(2):
+        e = r.experts[:, k].long().clamp(min=0)
+        gate = p.gather(1, e[:, None]) / sum(p.gather(1, r.experts[:, q].long().clamp(min=0)[:, None]) for q in range(2))
+        inner = torch.nn.functional.silu((x[:, None, :] * up[e].transpose(1, 2)).sum(2))
+        y = y + torch.where(mask[:, None], gate * (inner[:, None, :] * down[e].transpose(1, 2)).sum(2), 0.0)
+    counts = r.counts.float()
+    balance = 6 * (counts / counts.sum() * p[mask].mean(0)).sum()
+    want = torch.nn.functional.cross_entropy(y @ out.t(), target) + 0.01 * balance
+    want.backward()
+    assert abs(float(loss.detach()) - float(want.detach())) < 0.02 * float(want.detach())
+    for a, b in zip(model.parameters(), plain):
+        # bf16 activations and gradients at every step of the model: a few roundings of 2^-9 each.
+        assert float((a.grad.float() - b.grad).norm()) < 0.03 * float(b.grad.norm())
 
 
 def test_training_operators_refuse(ft):
