@@ -45,21 +45,20 @@ __device__ __forceinline__ void eachPack(const T* in, uint64_t begin, uint64_t e
 }
 
 // f(tensor, first element, past the last element) for the workgroup's chunks of the batch, from the
-// first to the last or back.
+// first to the last or back.  The lanes hold the tensors' first chunks, and a chunk's tensor is the last
+// that starts no later: kernel arguments are in host memory, where each step of a search of them waits
+// about a microsecond.
 template <class F>
 __device__ __forceinline__ void eachChunk(const Batch& b, bool back, F&& f) {
+    static_assert(kBatch <= 2 * kWave, "two tensors a lane");
+    const int lane      = threadIdx.x % kWave;
+    const uint32_t low  = lane < b.n ? b.first[lane] : UINT32_MAX;
+    const uint32_t high = lane + kWave < b.n ? b.first[lane + kWave] : UINT32_MAX;
     for (uint32_t c = blockIdx.x; c < b.chunks; c += gridDim.x) {
         const uint32_t chunk = back ? b.chunks - 1 - c : c;
-        int lo = 0, hi = b.n - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (b.first[mid] <= chunk)
-                lo = mid;
-            else
-                hi = mid - 1;
-        }
-        const uint64_t begin = static_cast<uint64_t>(chunk - b.first[lo]) * kChunk;
-        f(lo, begin, min(begin + kChunk, b.count[lo]));
+        const int t          = __popcll(__ballot(low <= chunk)) + __popcll(__ballot(high <= chunk)) - 1;
+        const uint64_t begin = static_cast<uint64_t>(chunk - b.first[t]) * kChunk;
+        f(t, begin, min(begin + kChunk, b.count[t]));
     }
 }
 

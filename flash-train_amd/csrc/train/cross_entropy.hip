@@ -308,7 +308,11 @@ struct Tiling {
 //     64 x 4096 x 128000 201 / 234; gradients of 500 x 1024 x 5003 77.6 / 60.2, 2048 x 4096 x 32003
 //     1198 / 1392;
 //   fp32, us, 128x128 / 64x64: loss of 300 x 8192 x 3000 470 / 166, 1000 x 1000 x 1000 80 / 36.
-double tileMicros(bool fp32, int rows, int cols, int64_t m, int64_t n, int64_t k, int slices) {
+double tileMicros(bool fp32, HeadTile what, int rows, int cols, int64_t m, int64_t n, int64_t k, int slices) {
+    // dw's 128x128 tiles run two to a CU: fp16 500 x 1024 x 5003 15.5 us against 16.4 on 256x256, bf16
+    // 200 x 4096 x 10000 47.9 against 41.5, 16 x 4096 x 32003 113 against 80.
+    if (what == HeadTile::kGradWeight && rows == 128)
+        return static_cast<double>(ceilDiv(ceilDiv(m, rows) * ceilDiv(n, cols), 2 * kCus)) * (static_cast<double>(k) / 64 * 0.8 + 10.0);
     const double stage = fp32 ? (rows == 128 ? 1.75 : 0.5) : rows == 256 ? (m <= 128 ? 0.75 : 1.25) : rows == 128 ? 0.5 : 0.3;
     const double ends  = fp32 ? 5.0 : rows == 256 ? 9.0 : 6.0;
     const uint64_t rounds = ceilDiv(ceilDiv(m, rows) * ceilDiv(n, cols) * slices, kCus);
@@ -334,7 +338,7 @@ Tiling tilingOf(FTrainNumericType type, HeadTile what, int64_t m, int64_t n, int
         const uint64_t tiles = std::max<uint64_t>(1, ceilDiv(m, rows) * ceilDiv(n, cols));
         const int most       = static_cast<int>(std::max<uint64_t>(1, std::min<uint64_t>(at_once * kCus / tiles, k / 512)));
         auto offer           = [&](int slices, double more) {
-            const double micros = tileMicros(fp32, rows, cols, m, n, k, slices) + more;
+            const double micros = tileMicros(fp32, what, rows, cols, m, n, k, slices) + more;
             if (best.rows == 0 || micros < least) {
                 best  = {rows, slices};
                 least = micros;

@@ -141,6 +141,7 @@ struct GradLogitsEnd16 {
     __device__ __forceinline__ void operator()(TileSums& acc, char* lds, int m0, int n0) const {
         typedef gemm::ppdev::u32x4 u32x4;
         typedef gemm::ppdev::u32x2 u32x2;
+        typedef gemm::ppdev::floatx4 floatx4;
         const Place at;
         const int rows_left = M - m0, cols_left = N - n0;
         RowInfo info[2][4];
@@ -149,26 +150,48 @@ struct GradLogitsEnd16 {
 #pragma unroll
             for (int u = 0; u < 4; ++u) info[i][u] = rows[m0 + min(at.row(i, u), rows_left - 1)];
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        auto value = [&](floatx4& x, int i, int u, int c, bool last) {
+            const RowInfo& r = info[i][u];
+            // exp(l - lse) as 2^(l log2 e - lse log2 e): the rounding of the second product, 2^-24 of it,
+            // is far below that of the result to 16 bits.
+            const float low = r.lse * -kLog2e, g = r.target < 0 ? NAN : r.grad;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], kLog2e, low)) * g;
+            if (last) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (c + e >= cols_left) x[e] = 0.f;
+            }
+        };
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             if (128 * i >= rows_left) break;
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const RowInfo r = info[i][u];
-                const int y     = r.target - first_class - n0;
-                const float g   = r.target < 0 ? NAN : r.grad;
-                char* const to  = lds + at.row(i, u) * 512;
+                const RowInfo& r = info[i][u];
+                if (cols_left >= 256) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) value(acc[i][q >> 1][u][q & 1], i, u, at.col(q >> 1, q & 1), false);
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) value(acc[i][q >> 1][u][q & 1], i, u, at.col(q >> 1, q & 1), true);
+                }
+                // The target's class, in the few tiles that hold it (a NaN stays one).
+                const int y   = r.target - first_class - n0;
+                const bool my = y >= 0 && y < min(256, cols_left) && ((y >> 5) & 3) == at.wn && ((y >> 2) & 3) == at.g;
+                if (__any(my)) {
+#pragma unroll
+                    for (int q = 0; q < 16; ++q)
+                        if (my && (y >> 7) == (q >> 3) && ((y >> 4) & 1) == ((q >> 2) & 1) && (y & 3) == (q & 3))
+                            acc[i][q >> 3][u][(q >> 2) & 1][q & 3] -= r.grad;
+                }
+                char* const to = lds + at.row(i, u) * 512;
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
                     for (int v = 0; v < 2; ++v) {
-                        const int c = at.col(j, v);
-                        float x[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            x[e] = (expFast(acc[i][j][u][v][e] - r.lse) - (c + e == y ? 1.f : 0.f)) * g;
-                            if (c + e >= cols_left) x[e] = 0.f;
-                        }
+                        const int c      = at.col(j, v);
+                        const floatx4& x = acc[i][j][u][v];
                         *reinterpret_cast<u32x2*>(to + 16 * ((c >> 3) ^ at.j16) + 8 * (at.g & 1)) =
                             u32x2{gemm::ppdev::pack2<BF16>(x[0], x[1]), gemm::ppdev::pack2<BF16>(x[2], x[3])};
                     }
@@ -308,6 +331,34 @@ struct GradLogitsEnd128 {
     }
 };
 
+// 16-bit dw: rows of any address.  (The tile's own end stores 2 bytes a lane.)
+template <bool BF16>
+struct GradWeightEnd128 {
+    using T = std::conditional_t<BF16, bf16, fp16>;
+    T* d;
+    int64_t ldd;
+    int M, N;
+    float alpha;
+
+    __device__ __forceinline__ void operator()(TileSums128<128>& acc, char* a, char* b, int m0, int n0) const {
+        const int rows_left = M - m0, cols_left = N - n0;
+        turned128<128>(acc, a, b, [&](int, int row, int col, float (&v)[8]) {
+            if (row >= rows_left || col >= cols_left) return;
+            T* const to = d + (m0 + row) * ldd + n0 + col;
+            Pack<T> out;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) out.v[e] = static_cast<T>(v[e] * alpha);
+            if (col + 8 <= cols_left) {
+                *reinterpret_cast<Pack<T>*>(to) = out;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 7; ++e)
+                    if (col + e < cols_left) to[e] = out.v[e];
+            }
+        });
+    }
+};
+
 // ---- fp32: the tiles of gemm/dma32_tile.hpp, four adjacent sums of a row at a time.
 
 // A row's largest logit and sum of exponentials over the 64 classes that 16 lanes hold.
@@ -433,13 +484,12 @@ __global__ __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_pe
 // ROTATE: neighbouring column tiles start at different stages, or all workgroups would read the same few
 // HBM channels at once where the weight's rows are a power of two apart.
 template <bool BF16, HeadTile WHAT, int BM>
-__global__ __launch_bounds__(256, BM == 64 ? 2 : 1) void headTileHalf128(HeadTileArgs h) {
+__global__ __launch_bounds__(256, BM == 64 || WHAT == HeadTile::kGradWeight ? 2 : 1) void headTileHalf128(HeadTileArgs h) {
     using T = std::conditional_t<BF16, bf16, fp16>;
     gemm::HalfGemmParams p{};
     if (!tileProblem<WHAT>(h, p, BM, 128)) return;
     p.a = h.a, p.b = h.b, p.d = h.d;
     using gemm::ddev::half_gemm_dma_tile;
-    using gemm::ddev::StoreTile;
     if constexpr (WHAT == HeadTile::kLogSum) {
         using End = LogSumEnd128<BM>;
         half_gemm_dma_tile<BF16, false, true, 128, false, BM, 3, true, End>(
@@ -464,9 +514,10 @@ __global__ __launch_bounds__(256, BM == 64 ? 2 : 1) void headTileHalf128(HeadTil
         p.d             = static_cast<float*>(h.d) + blockIdx.z * h.slice;
         half_gemm_dma_tile<BF16, false, true, 128, false, BM, 3, true>(p, blockIdx.x);
     } else {
-        p.alpha   = h.head->inv_scale;
-        p.cd_half = 1;
-        half_gemm_dma_tile<BF16, true, false, 128, false, 128, 3>(p, blockIdx.x, 0, 8, StoreTile{}, h.read_m, h.read_n);
+        // Two stage buffers, two workgroups to a CU: k, the tokens, is short.
+        using End = GradWeightEnd128<BF16>;
+        half_gemm_dma_tile<BF16, true, false, 128, false, 128, 2, false, End>(
+            p, blockIdx.x, 0, 8, End{static_cast<T*>(h.d), h.ldd, p.m, p.n, h.head->inv_scale}, h.read_m, h.read_n);
     }
 }
 

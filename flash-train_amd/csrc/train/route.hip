@@ -186,24 +186,23 @@ struct Candidates {
     }
 };
 
-// What `choose` and `place` keep in LDS, one after the other.
-union RouteLds {
-    struct {
-        int hist[kMaxExperts];
-        float sums[kThreads * 16];
-        int routed[kThreads];
-    } choose;
-    struct {
-        int first[kMaxExperts];         // slot of the workgroup's first choice of each expert
-        int next[kWaves][kMaxExperts];  // each wave's choices, then its next slot
-    } place;
+// What `choose` and `place` keep in LDS (one workgroup may do both, one after the other).
+struct ChooseLds {
+    int hist[kMaxExperts];
+    float sums[kThreads * 16];
+    int routed[kThreads];
+};
+template <int THREADS>
+struct PlaceLds {
+    int first[kMaxExperts];                   // slot of the workgroup's first choice of each expert
+    int next[THREADS / kWave][kMaxExperts];  // each wave's choices, then its next slot
 };
 
 template <class T, int VPL, int G, bool VEC>
-__device__ __forceinline__ void chooseRows(const RouteArgs& a, RouteLds& lds) {
+__device__ __forceinline__ void chooseRows(const RouteArgs& a, ChooseLds& lds) {
     constexpr int kRows = kThreads / G;  // rows at a time
-    int* const hist   = lds.choose.hist;
-    float* const sums = lds.choose.sums;
+    int* const hist   = lds.hist;
+    float* const sums = lds.sums;
     const int group = threadIdx.x / G, n = a.n_experts;
     Row<T, VPL, G, VEC> row;
     row.g = threadIdx.x % G;
@@ -275,7 +274,7 @@ __device__ __forceinline__ void chooseRows(const RouteArgs& a, RouteLds& lds) {
     }
 #pragma unroll
     for (int j = 0; j < VPL; ++j) sums[group * (G * VPL) + row.index(j)] = sum_p[j];
-    if (row.g == 0) lds.choose.routed[group] = routed;
+    if (row.g == 0) lds.routed[group] = routed;
     __syncthreads();
     for (int e = threadIdx.x; e < n; e += kThreads) {
         float s = 0.f;
@@ -285,13 +284,15 @@ __device__ __forceinline__ void chooseRows(const RouteArgs& a, RouteLds& lds) {
     }
     if (threadIdx.x == 0) {
         int s = 0;
-        for (int r = 0; r < kRows; ++r) s += lds.choose.routed[r];
+        for (int r = 0; r < kRows; ++r) s += lds.routed[r];
         a.block_routed[blockIdx.x] = s;
     }
 }
 
 // Exclusive prefix sum of one value a thread over the workgroup; total: the sum.
+template <int THREADS = kThreads>
 __device__ __forceinline__ int blockScan(int v, int& total) {
+    constexpr int kWaves = THREADS / kWave;
     __shared__ int wave_sum[kWaves];
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     int s = v;
@@ -314,54 +315,71 @@ __device__ __forceinline__ int blockScan(int v, int& total) {
 }
 
 // Of kScanExperts experts: each workgroup's first rank in place of its count, the expert's count, its sum
-// of p.  Adjacent threads take adjacent experts, each a run of the workgroups.
-constexpr int kScanExperts = 8;
-__global__ __launch_bounds__(kThreads) void scan(RouteArgs a) {
-    constexpr int kRuns = kThreads / kScanExperts;
-    __shared__ int counts[kRuns][kScanExperts];
-    __shared__ float sums[kRuns][kScanExperts];
+// of p.  Adjacent threads take adjacent experts, each a run of the workgroups; runs are joined in groups.
+constexpr int kScanExperts = 8, kScanThreads = 1024, kScanGroup = 8;
+__global__ __launch_bounds__(kScanThreads) void scan(RouteArgs a) {
+    constexpr int kRuns = kScanThreads / kScanExperts, kGroups = kRuns / kScanGroup;
+    constexpr int kPer = kMaxBlocks / kRuns;
+    __shared__ int counts[kRuns][kScanExperts], groups[kGroups][kScanExperts];
+    __shared__ float sums[kRuns][kScanExperts], group_sums[kGroups][kScanExperts];
     const int n = a.n_experts, run = threadIdx.x / kScanExperts, i = threadIdx.x % kScanExperts;
-    const int e = blockIdx.x * kScanExperts + i, per = (a.blocks + kRuns - 1) / kRuns;
-    const int first = run * per, last = e < n ? min(first + per, a.blocks) : first;
+    const int e = blockIdx.x * kScanExperts + i, first = run * kPer;
     int32_t* const count = a.block_count + e;
     const float* const p = a.block_p + e;
-    int c                = 0;
-    float sum            = 0.f;
-#pragma unroll 8
-    for (int b = first; b < last; ++b) {
-        c += count[static_cast<int64_t>(b) * n];
-        sum += p[static_cast<int64_t>(b) * n];
+    int mine[kPer], c = 0;
+    float sum = 0.f;
+#pragma unroll
+    for (int b = 0; b < kPer; ++b) {
+        const bool in = e < n && first + b < a.blocks;
+        mine[b]       = in ? count[static_cast<int64_t>(first + b) * n] : 0;
+        sum += in ? p[static_cast<int64_t>(first + b) * n] : 0.f;
     }
+#pragma unroll
+    for (int b = 0; b < kPer; ++b) c += mine[b];
     counts[run][i] = c;
     sums[run][i]   = sum;
     __syncthreads();
-    int before = 0;
-    for (int r = 0; r < run; ++r) before += counts[r][i];
+    if (run < kGroups) {
+        int all   = 0;
+        float sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < kScanGroup; ++r) {
+            all += counts[run * kScanGroup + r][i];
+            sum += sums[run * kScanGroup + r][i];
+        }
+        groups[run][i]     = all;
+        group_sums[run][i] = sum;
+    }
+    __syncthreads();
+    const int group = run / kScanGroup;
+    int before      = 0;
+    for (int q = 0; q < group; ++q) before += groups[q][i];
+    for (int r = group * kScanGroup; r < run; ++r) before += counts[r][i];
     if (run == kRuns - 1 && e < n) {
         float all = 0.f;
-        for (int r = 0; r < kRuns; ++r) all += sums[r][i];
+        for (int q = 0; q < kGroups; ++q) all += group_sums[q][i];
         a.counts[e] = before + c;
         a.sum_p[e]  = all;
     }
-#pragma unroll 8
-    for (int b = first; b < last; ++b) {
-        const int x                         = count[static_cast<int64_t>(b) * n];
-        count[static_cast<int64_t>(b) * n] = before;
-        before += x;
+#pragma unroll
+    for (int b = 0; b < kPer; ++b) {
+        if (e < n && first + b < a.blocks) count[static_cast<int64_t>(first + b) * n] = before;
+        before += mine[b];
     }
 }
 
 // The slots of the workgroup's choices; workgroup 0 also finishes the loss.  SCANNED: `scan` has run;
 // else every workgroup adds up the others' counts by itself.
-template <bool SCANNED>
-__device__ __forceinline__ void placeRows(const RouteArgs& a, RouteLds& lds) {
-    int* const first = lds.place.first;
-    auto& next       = lds.place.next;
+template <bool SCANNED, int THREADS>
+__device__ __forceinline__ void placeRows(const RouteArgs& a, PlaceLds<THREADS>& lds) {
+    constexpr int kThreads = THREADS, kWaves = THREADS / kWave;
+    int* const first = lds.first;
+    auto& next       = lds.next;
     const int n = a.n_experts, lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     if constexpr (!SCANNED) {
         // A thread an expert, or several: adjacent threads adjacent experts, each with the workgroups
         // from `part` on in steps of `parts`.
-        const int parts = n <= kThreads / 4 ? 4 : n <= kThreads / 2 ? 2 : 1;
+        const int parts = n <= kThreads / 8 ? 8 : n <= kThreads / 2 ? 2 : 1;
         const int part = threadIdx.x / (kThreads / parts), self = blockIdx.x;
         __shared__ int all_of[kThreads], before_of[kThreads];
         __shared__ float sum_of[kThreads];
@@ -411,8 +429,8 @@ __device__ __forceinline__ void placeRows(const RouteArgs& a, RouteLds& lds) {
             dot += static_cast<float>(c) * (SCANNED ? a.sum_p[e] : __builtin_bit_cast(float, next[2][e]));
         }
         int all_routed, all;
-        (void)blockScan(routed, all_routed);
-        (void)blockScan(total, all);
+        (void)blockScan<THREADS>(routed, all_routed);
+        (void)blockScan<THREADS>(total, all);
         dot = groupSum<kWave>(dot);
         if (lane == 0) part[wave] = dot;
         __syncthreads();
@@ -426,7 +444,7 @@ __device__ __forceinline__ void placeRows(const RouteArgs& a, RouteLds& lds) {
     for (int e0 = 0; e0 < n; e0 += kThreads) {
         const int e = e0 + threadIdx.x;
         int total;
-        const int at = blockScan(e < n ? count_of(e) : 0, total);
+        const int at = blockScan<THREADS>(e < n ? count_of(e) : 0, total);
         if (e < n)
             first[e] = before + at +
                        (SCANNED ? a.block_count[static_cast<int64_t>(blockIdx.x) * n + e] : next[1][e]);
@@ -477,18 +495,24 @@ __device__ __forceinline__ void placeRows(const RouteArgs& a, RouteLds& lds) {
 // One workgroup that has all rows goes on to place them.
 template <class T, int VPL, int G, bool VEC>
 __global__ __launch_bounds__(kThreads) void choose(RouteArgs a) {
-    __shared__ RouteLds lds;
-    chooseRows<T, VPL, G, VEC>(a, lds);
+    __shared__ union {
+        ChooseLds choose;
+        PlaceLds<kThreads> place;
+    } lds;
+    chooseRows<T, VPL, G, VEC>(a, lds.choose);
     if (a.blocks > 1) return;
     // The workgroup's own stores are there for it after the barrier.
     __syncthreads();
-    placeRows<false>(a, lds);
+    placeRows<false, kThreads>(a, lds.place);
 }
 
+// 131072 x 256, top 8 (16384 x 64, top 2): 8.3 us (8.1) with 256 threads, 7.4 (6.9) with 512, 10.8 (10.7)
+// with 1024.
+constexpr int kPlaceThreads = 512;
 template <bool SCANNED>
-__global__ __launch_bounds__(kThreads) void place(RouteArgs a) {
-    __shared__ RouteLds lds;
-    placeRows<SCANNED>(a, lds);
+__global__ __launch_bounds__(kPlaceThreads) void place(RouteArgs a) {
+    __shared__ PlaceLds<kPlaceThreads> lds;
+    placeRows<SCANNED, kPlaceThreads>(a, lds);
 }
 
 template <class T, int VPL, int G, bool VEC>
@@ -682,10 +706,10 @@ void moeRouteForward(const MoeRoute& p, void* workspace, hipStream_t stream) {
     launch(kernel, "router choose", dim3(a.blocks), dim3(kThreads), stream, a);
     if (a.blocks == 1) return;
     if (scanned) {
-        launch(&scan, "router scan", dim3(static_cast<uint32_t>(ceilDiv(a.n_experts, kScanExperts))), dim3(kThreads), stream, a);
-        launch(&place<true>, "router place", dim3(a.blocks), dim3(kThreads), stream, a);
+        launch(&scan, "router scan", dim3(static_cast<uint32_t>(ceilDiv(a.n_experts, kScanExperts))), dim3(kScanThreads), stream, a);
+        launch(&place<true>, "router place", dim3(a.blocks), dim3(kPlaceThreads), stream, a);
     } else {
-        launch(&place<false>, "router place", dim3(a.blocks), dim3(kThreads), stream, a);
+        launch(&place<false>, "router place", dim3(a.blocks), dim3(kPlaceThreads), stream, a);
     }
 }
 
