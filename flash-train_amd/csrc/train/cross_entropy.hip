@@ -290,8 +290,10 @@ __global__ __launch_bounds__(kThreads) void finishHidden(const float* sums, int6
 uint64_t ceilDiv(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 uint64_t roundUp(uint64_t a, uint64_t b) { return ceilDiv(a, b) * b; }
 
-// Bytes of a piece of dl: the last-level cache's 256 MiB, which it is read from twice.
-constexpr uint64_t kPieceBytes = 256ull << 20;
+// Bytes of a piece of dl.  Small pieces fill the device badly and add dx up more often; 8192 x 4096 x
+// 131072 (16384 x 2048 x 65536) bf16 gradients, us, at 64 MiB 18494 (13042), 128 17655 (10997), 256 17507
+// (9380), 512 17371 (9234), 1024 17256 (9204).
+constexpr uint64_t kPieceBytes = 512ull << 20;
 constexpr uint64_t kCus = 256;
 
 // How a product runs: tile rows (launchHeadTile), and slices of k that keep sums of their own.
