@@ -13,11 +13,12 @@
 // stay in registers and cross the group by lane permutations.  With many experts vector instructions
 // bound the choice, 131072 x 256 fp32, top 8: pairs of value and index reduced by shuffles 148 us,
 // maxima first and then the place by a ballot 109, on whole numbers 87 (eight a lane), 59 (16 a lane: the
-// steps across lanes serve four rows of a wave instead of two).  A workgroup takes a run of
-// consecutive rows, so the order of the choices within an expert is the order of (workgroup, row,
-// rank): `choose` counts each workgroup's choices, `scan` turns them into each workgroup's first
-// rank (one workgroup per expert), `place` hands out the slots.  Sums over rows are taken in a fixed
-// order; the only atomics count in LDS, in whole numbers.
+// steps across lanes serve four rows of a wave instead of two), 55 with the numbers in LDS, 44 with the
+// next row's loads under way and the numbers in 16-byte writes to different banks (3.0 TB/s; the reads
+// alone would be 27 us).  A workgroup takes a run of consecutive rows, so the order of the choices within
+// an expert is the order of (workgroup, row, rank): `choose` counts each workgroup's choices, `scan` turns
+// them into each workgroup's first rank (one workgroup per expert), `place` hands out the slots.  Sums
+// over rows are taken in a fixed order; the only atomics count in LDS, in whole numbers.
 #include <algorithm>
 
 #include "device.hpp"
@@ -29,7 +30,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves   = kThreads / kWave;
 constexpr int kCus     = 256;
-// Most workgroups.
+// Most workgroups: as many as are on the chip at once with the registers of the widest rows.  Six a CU:
+// choose 46.8, scan 9.7 and place 10.0 us at 131072 x 256 instead of 44.3, 7.6 and 7.7.
 constexpr int kMaxBlocks = 4 * kCus;
 // Which form the forward pass takes (moeRouteForward): passes of one workgroup over rows, and counts.
 constexpr uint64_t kWholePasses = 4, kScanPasses = 8, kScanCounts = 32768;
@@ -66,25 +68,32 @@ struct Row {
 #pragma unroll
         for (int j = 0; j < VPL; ++j) v[j] = -INFINITY;
     }
-    __device__ __forceinline__ void load(const T* row, int n) {
+    // fetch: the loads alone, of what unpack makes logits of.
+    static constexpr int kVec = 16 / sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(kVec)));
+    vec raw[VEC ? VPL / kVec : 1];
+    T one[VEC ? 1 : VPL];
+    __device__ __forceinline__ void fetch(const T* row, int n) {
         if constexpr (VEC) {
-            constexpr int N = 16 / sizeof(T);
 #pragma unroll
-            for (int j = 0; j < VPL; j += N) {
-                if (index(j) < n) {
-                    typedef T vec __attribute__((ext_vector_type(N)));
-                    const vec x = *reinterpret_cast<const vec*>(row + index(j));
-#pragma unroll
-                    for (int e = 0; e < N; ++e) v[j + e] = toFloat(static_cast<T>(x[e]));
-                } else {
-#pragma unroll
-                    for (int e = 0; e < N; ++e) v[j + e] = -INFINITY;
-                }
-            }
+            for (int j = 0; j < VPL; j += kVec)
+                if (index(j) < n) raw[j / kVec] = *reinterpret_cast<const vec*>(row + index(j));
         } else {
 #pragma unroll
-            for (int j = 0; j < VPL; ++j) v[j] = index(j) < n ? toFloat(row[index(j)]) : -INFINITY;
+            for (int j = 0; j < VPL; ++j)
+                if (index(j) < n) one[j] = row[index(j)];
         }
+    }
+    __device__ __forceinline__ void unpack(int n) {
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+            const T x = VEC ? static_cast<T>(raw[VEC ? j / kVec : 0][j % kVec]) : one[VEC ? 0 : j];
+            v[j]      = index(VEC ? j / kVec * kVec : j) < n ? toFloat(x) : -INFINITY;
+        }
+    }
+    __device__ __forceinline__ void load(const T* row, int n) {
+        fetch(row, n);
+        unpack(n);
     }
     // Exponentials relative to `top` into p; their sum is returned: 0 only where every logit is minus
     // infinity (a NaN makes it NaN).
@@ -111,17 +120,32 @@ __device__ __forceinline__ unsigned maxOf(unsigned a, unsigned b) { return a > b
 // The logits as whole numbers in their order, from which the largest are taken one by one (0: taken; a
 // NaN counts as minus infinity, which is never chosen; the two zeros are one).  Integers, because a
 // floating maximum of values that may be NaN takes two more instructions to make them quiet, at every
-// step.
-//   A 16-bit logit leaves 13 bits of its number free: they hold 1023 less its index, so the largest
-// number is the largest logit with the lowest index, and nothing else need be found out.
+// step.  What a step costs is vector instructions of every lane for the one that holds the largest:
+//   kPacked: a 16-bit logit leaves 13 bits of its number free, which hold 1023 less its index; the
+// largest number is the largest logit with the lowest index, and each lane strikes it from its own.
+//   kShared (16 logits a lane, or fp32 with lanes enough): the numbers lie in LDS in the row's order, a
+// lane keeps the maximum of its run of them.  The lowest lane with the largest is found by a ballot, and
+// the whole group reads that lane's run, one number each: a ballot finds the place, a maximum over the
+// lanes is the run's next.
+//   Otherwise (few lanes) the lowest index of those that are equal to the largest.
 template <class T, int VPL, int G, bool VEC>
 struct Candidates {
-    static constexpr bool kPacked    = sizeof(T) == 2;
+    static constexpr bool kPacked    = sizeof(T) == 2 && VPL == 8;
+    static constexpr bool kShared    = !kPacked && G >= VPL;
     static constexpr unsigned kIndex = kMaxExperts - 1, kFree = 0x1FFFu;
     static constexpr unsigned kLeast = 0x00800000u;  // the number of the lowest finite value is not less
+    // Words of a row in LDS: the rows of a wave start in different banks.  A lane's run lies in 16-byte
+    // chunks, chunk c at place (c + lane / 4) mod 4 of every four, so that lanes write to different banks.
+    static constexpr int kStride = G * VPL + 16;
+    static __device__ __forceinline__ int placeOf(int run, int j) {
+        constexpr int kMask = VPL / 4 - 1 < 3 ? VPL / 4 - 1 : 3;
+        return run * VPL + 4 * ((j / 4 & ~kMask) | ((j / 4 + run / 4) & kMask)) + j % 4;
+    }
     unsigned key[VPL];
+    unsigned own;          // the lane's largest
+    unsigned* const row_;  // kShared: the row's numbers
 
-    __device__ __forceinline__ explicit Candidates(const Row<T, VPL, G, VEC>& row) {
+    __device__ __forceinline__ Candidates(const Row<T, VPL, G, VEC>& row, unsigned* lds) : row_(lds + threadIdx.x / G * kStride) {
 #pragma unroll
         for (int j = 0; j < VPL; ++j) {
             const unsigned bits = __builtin_bit_cast(unsigned, fmaxf(row.v[j] + 0.f, -INFINITY));
@@ -129,6 +153,27 @@ struct Candidates {
             if constexpr (kPacked) k = (k & ~kFree) | (kIndex - row.index(j));
             key[j] = k;
         }
+        if constexpr (kShared) {
+            waveFence();  // the wave is done with the rows before
+            typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+            if constexpr (VEC) {
+#pragma unroll
+                for (int j = 0; j < VPL; j += 4)
+                    *reinterpret_cast<u32x4*>(row_ + placeOf(row.g, j)) = u32x4{key[j], key[j + 1], key[j + 2], key[j + 3]};
+            } else {
+#pragma unroll
+                for (int j = 0; j < VPL; ++j) row_[placeOf(row.index(j) / VPL, row.index(j) % VPL)] = key[j];
+                waveFence();
+#pragma unroll
+                for (int j = 0; j < VPL; j += 4) {
+                    const u32x4 x = *reinterpret_cast<const u32x4*>(row_ + placeOf(row.g, j));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) key[j + e] = x[e];
+                }
+            }
+            waveFence();
+        }
+        own = mine();
     }
     __device__ __forceinline__ unsigned mine() const {
         unsigned m = key[0];
@@ -137,41 +182,41 @@ struct Candidates {
         return m;
     }
     // The group's largest number.
-    __device__ __forceinline__ unsigned best(unsigned own) const {
-        return groupReduce<G>(own, [](unsigned a, unsigned b) { return maxOf(a, b); });
+    __device__ __forceinline__ unsigned best() const { return largest(own); }
+    static __device__ __forceinline__ unsigned largest(unsigned v) {
+        return groupReduce<G>(v, [](unsigned a, unsigned b) { return maxOf(a, b); });
     }
     static __device__ __forceinline__ float value(unsigned k) {
         if (k < kLeast) return -INFINITY;
         if constexpr (kPacked) k = (k & 0x80000000u) ? k & ~kFree : k | kFree;
         return __builtin_bit_cast(float, (k & 0x80000000u) ? k ^ 0x80000000u : ~k);
     }
-    // Takes out the largest, `best`; returns its index.  own: mine().
-    __device__ __forceinline__ int take(unsigned best, unsigned own, const Row<T, VPL, G, VEC>& row) {
+    // The lowest lane of the group for which `is` holds (for one it does).
+    static __device__ __forceinline__ int lowestLane(bool is, int g) {
+        const unsigned long long all = __ballot(is);
+        if constexpr (G == kWave) return __builtin_ctzll(all);
+        const int first = threadIdx.x % kWave - g;
+        if constexpr (G == 32) return __builtin_ctz(static_cast<unsigned>(first == 0 ? all : all >> 32));
+        return __builtin_ctz(static_cast<unsigned>(all >> first));
+    }
+    // Takes out the largest, `best`; returns its index.
+    __device__ __forceinline__ int take(unsigned best, const Row<T, VPL, G, VEC>& row) {
         if constexpr (kPacked) {
 #pragma unroll
             for (int j = 0; j < VPL; ++j) key[j] = key[j] == best ? 0u : key[j];
+            own = mine();
             return kIndex - (best & kIndex);
-        } else if constexpr (VEC) {
-            // Lanes hold their logits in the row's order: of those that tie, the lowest lane has the
-            // lowest index.
-            bool open = own == best;
-            int from  = 0;
-            if constexpr (G > 1) {
-                const unsigned long long all = __ballot(open);
-                const int lane = threadIdx.x % kWave, first = lane - row.g;
-                const unsigned long long group = G == kWave ? all : (all >> first) & ((1ull << (G % kWave)) - 1ull);
-                from = first + __builtin_ctzll(group);
-                open = open && from == lane;
-            }
-            int found = 0;
-#pragma unroll
-            for (int j = 0; j < VPL; ++j) {
-                const bool hit = open && key[j] == best;
-                found          = hit ? row.index(j) : found;
-                key[j]         = hit ? 0u : key[j];
-                open           = open && !hit;
-            }
-            return G > 1 ? __shfl(found, from, kWave) : found;
+        } else if constexpr (kShared) {
+            const int from = lowestLane(own == best, row.g);
+            unsigned* const mine = row_ + placeOf(from, row.g % VPL);
+            unsigned x           = row.g < VPL ? *mine : 0u;
+            const int j          = lowestLane(x == best && row.g < VPL, row.g);
+            x                    = row.g == j ? 0u : x;
+            if (row.g == j) *mine = 0u;
+            waveFence();
+            const unsigned next = largest(x);
+            own                 = row.g == from ? next : own;
+            return from * VPL + j;
         } else {
             int found = INT32_MAX;
 #pragma unroll
@@ -181,6 +226,7 @@ struct Candidates {
 #pragma unroll
             for (int j = 0; j < VPL; ++j)
                 if (row.index(j) == at) key[j] = 0u;
+            own = mine();
             return at;
         }
     }
@@ -189,7 +235,10 @@ struct Candidates {
 // What `choose` and `place` keep in LDS (one workgroup may do both, one after the other).
 struct ChooseLds {
     int hist[kMaxExperts];
-    float sums[kThreads * 16];
+    union {
+        alignas(16) unsigned rows[kThreads * 16 + kThreads];  // Candidates: at most 32 rows, 16 words apart
+        float sums[kThreads * 16];                            // after them
+    };
     int routed[kThreads];
 };
 template <int THREADS>
@@ -213,16 +262,24 @@ __device__ __forceinline__ void chooseRows(const RouteArgs& a, ChooseLds& lds) {
     int routed       = 0;
     const int64_t first = static_cast<int64_t>(blockIdx.x) * a.rows_per_block;
     const int64_t last  = min(first + a.rows_per_block, a.rows);
+    // The next row's loads are under way while a row is worked on.
+    bool kept        = false;
+    const auto fetch = [&](int64_t t) {
+        if (t >= last) return;
+        kept = a.mask == nullptr || a.mask[t] != 0;
+        row.fetch(static_cast<const T*>(a.logits) + t * a.ld, n);
+    };
+    fetch(first + group);
     for (int64_t t = first + group; t < last; t += kRows) {
-        const bool kept = a.mask == nullptr || a.mask[t] != 0;
         int32_t* const experts = a.experts + t * a.top_k;
         float* const gates     = a.gates + t * a.top_k;
         if (kept)
-            row.load(static_cast<const T*>(a.logits) + t * a.ld, n);
+            row.unpack(n);
         else
             row.clear();
-        Candidates<T, VPL, G, VEC> left(row);
-        unsigned own = left.mine(), best = left.best(own);
+        fetch(t + kRows);
+        Candidates<T, VPL, G, VEC> left(row, lds.rows);
+        unsigned best   = left.best();
         const float top = left.value(best);
         float p[VPL];
         const float total = row.exponentials(p, top);
@@ -248,10 +305,9 @@ __device__ __forceinline__ void chooseRows(const RouteArgs& a, ChooseLds& lds) {
             if (s * G >= a.top_k) continue;
             unsigned number = 0;
             for (int k = 0; k < G && s * G + k < a.top_k; ++k) {
-                const int e = left.take(best, own, row);
+                const int e = left.take(best, row);
                 if (k == row.g) at[s] = best >= left.kLeast ? e : INT32_MAX, number = best;
-                own  = left.mine();
-                best = left.best(own);
+                best = left.best();
             }
             // A row whose sum is NaN has NaN gates.
             gate[s] = at[s] < n ? expExact(left.value(number) - top) * inv : 0.f;
@@ -272,6 +328,7 @@ __device__ __forceinline__ void chooseRows(const RouteArgs& a, ChooseLds& lds) {
             }
         }
     }
+    __syncthreads();
 #pragma unroll
     for (int j = 0; j < VPL; ++j) sums[group * (G * VPL) + row.index(j)] = sum_p[j];
     if (row.g == 0) lds.routed[group] = routed;
