@@ -4,6 +4,7 @@
 
 #include <vector>
 
+#include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
@@ -39,6 +40,14 @@ FTrainStorageView view(const Tensor& t, const char* name) {
                              false};
 }
 
+// A tensor of one value as an array of one.
+FTrainStorageView viewOne(const Tensor& t, const char* name) {
+    static const int64_t one = 1;
+    FTrainStorageView v      = view(t, name);
+    v.dims = &one, v.strides = nullptr, v.num_dims = 1;
+    return v;
+}
+
 FTrainStorageView none() {
     static const int64_t zero = 0;
     return FTrainStorageView{nullptr, &zero, nullptr, 1, FTRAIN_NUMERIC_TYPE_UINT8, FTRAIN_INDEX_TYPE_CONTINUOUS, false};
@@ -52,14 +61,19 @@ void check(FTrainStatus status, const char* what) {
 // The device of a call: its guard, its current stream, and tensors made on it.
 class Call {
   public:
-    explicit Call(const Tensor& t, const char* name) : options_(t.options()), guard_(deviceOf(t, name)) {
-        stream_ = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream();
+    explicit Call(const Tensor& t, const char* name) : device_(deviceOf(t, name)), guard_(device_) {
+        stream_ = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(device_.index()).stream();
     }
     void same(const Tensor& t, const char* name) const {
-        TORCH_CHECK(t.is_cuda() && t.device() == options_.device(), name, " must be on the device of the other tensors");
+        TORCH_CHECK(t.is_cuda() && t.device() == device_, name, " must be on the device of the other tensors");
     }
-    Tensor make(at::IntArrayRef sizes, at::ScalarType type) const { return torch::empty(sizes, options_.dtype(type)); }
-    Tensor workspace(uint64_t bytes) const { return make({static_cast<int64_t>(bytes)}, at::kByte); }
+    // An output.  Made below the dispatcher, and the workspace below tensors: a call of the router on few
+    // tokens is bound by the host, on which torch::empty takes 1 us.
+    Tensor make(at::IntArrayRef sizes, at::ScalarType type) const {
+        return Tensor(at::detail::empty_cuda(sizes, type, device_, c10::nullopt));
+    }
+    // Memory of the current stream, as a tensor's is.
+    c10::DataPtr workspace(uint64_t bytes) const { return c10::GetAllocator(c10::kCUDA)->allocate(bytes); }
     hipStream_t stream() const { return stream_; }
 
   private:
@@ -67,7 +81,7 @@ class Call {
         TORCH_CHECK(t.is_cuda(), name, " must be a device tensor");
         return t.device();
     }
-    at::TensorOptions options_;
+    c10::Device device_;
     c10::hip::HIPGuardMasqueradingAsCUDA guard_;
     hipStream_t stream_;
 };
@@ -95,9 +109,9 @@ std::tuple<Tensor, Tensor> crossEntropyForward(const Tensor& hidden_, const Tens
     uint64_t bytes = 0;
     check(ftrainLinearCrossEntropyWorkspaceBytes(view(hidden, "hidden"), view(weight, "weight"), false, &bytes),
           "ftrainLinearCrossEntropyWorkspaceBytes");
-    const Tensor workspace = call.workspace(bytes);
+    const c10::DataPtr workspace = call.workspace(bytes);
     check(ftrainLinearCrossEntropy(view(hidden, "hidden"), view(weight, "weight"), view(target, "target"),
-                                   view(loss, "loss"), view(lse, "lse"), ignore_index, workspace.data_ptr(), bytes,
+                                   view(loss, "loss"), view(lse, "lse"), ignore_index, workspace.get(), bytes,
                                    call.stream()),
           "ftrainLinearCrossEntropy");
     return {loss, lse};
@@ -120,10 +134,10 @@ std::tuple<Tensor, Tensor> crossEntropyBackward(const Tensor& grad_loss_, const 
     uint64_t bytes     = 0;
     check(ftrainLinearCrossEntropyWorkspaceBytes(view(hidden, "hidden"), view(weight, "weight"), true, &bytes),
           "ftrainLinearCrossEntropyWorkspaceBytes");
-    const Tensor workspace = call.workspace(bytes);
+    const c10::DataPtr workspace = call.workspace(bytes);
     check(ftrainLinearCrossEntropyBackward(view(grad_loss, "grad_loss"), view(hidden, "hidden"), view(weight, "weight"),
                                            view(target, "target"), view(lse, "lse"), view(grad_hidden, "grad_hidden"),
-                                           view(grad_weight, "grad_weight"), ignore_index, workspace.data_ptr(), bytes,
+                                           view(grad_weight, "grad_weight"), ignore_index, workspace.get(), bytes,
                                            call.stream()),
           "ftrainLinearCrossEntropyBackward");
     return {grad_hidden, grad_weight};
@@ -150,15 +164,15 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> routeForward(const Te
     TORCH_CHECK(!mask.has_value() || (mask->dim() == 1 && mask->size(0) == rows), "mask must hold one value a row");
     Tensor experts = call.make({rows, top_k}, at::kInt), gates = call.make({rows, top_k}, at::kFloat);
     Tensor slots = call.make({rows, top_k}, at::kInt), counts = call.make({n}, at::kInt);
-    Tensor routed = call.make({1}, at::kInt), loss = call.make({1}, at::kFloat);
+    Tensor routed = call.make({1}, at::kInt), loss = call.make({}, at::kFloat);
     uint64_t bytes = 0;
     check(ftrainMoeRouteWorkspaceBytes(view(logits, "logits"), &bytes), "ftrainMoeRouteWorkspaceBytes");
-    const Tensor workspace = call.workspace(bytes);
+    const c10::DataPtr workspace = call.workspace(bytes);
     check(ftrainMoeRoute(view(logits, "logits"), mask_view, view(experts, "experts"), view(gates, "gates"),
-                         view(slots, "slots"), view(counts, "counts"), view(routed, "routed"), view(loss, "loss"), normalize,
-                         workspace.data_ptr(), bytes, call.stream()),
+                         view(slots, "slots"), view(counts, "counts"), view(routed, "routed"), viewOne(loss, "loss"), normalize,
+                         workspace.get(), bytes, call.stream()),
           "ftrainMoeRoute");
-    return {experts, gates, slots, counts, routed, loss.squeeze(0)};
+    return {experts, gates, slots, counts, routed, loss};
 }
 
 Tensor routeBackward(const Tensor& grad_gates_, const Tensor& grad_loss_, const Tensor& logits_, const Tensor& experts_,
@@ -171,12 +185,11 @@ Tensor routeBackward(const Tensor& grad_gates_, const Tensor& grad_loss_, const 
     const Tensor logits = withRows(logits_), experts = experts_.contiguous(), counts = counts_.contiguous();
     const Tensor grad_gates = grad_gates_.contiguous(), routed = routed_.contiguous();
     TORCH_CHECK(grad_loss_.numel() == 1, "grad_loss must hold one value");
-    const Tensor grad_loss = grad_loss_.reshape({1});
     Tensor mask_dense;
     const FTrainStorageView mask_view = maskView(call, mask, mask_dense);
     TORCH_CHECK(!mask.has_value() || (mask->dim() == 1 && mask->size(0) == logits.size(0)), "mask must hold one value a row");
     Tensor grad_logits = call.make(logits.sizes(), logits.scalar_type());
-    check(ftrainMoeRouteBackward(view(grad_gates, "grad_gates"), view(grad_loss, "grad_loss"), view(logits, "logits"), mask_view,
+    check(ftrainMoeRouteBackward(view(grad_gates, "grad_gates"), viewOne(grad_loss_, "grad_loss"), view(logits, "logits"), mask_view,
                                  view(experts, "experts"), view(counts, "counts"), view(routed, "routed"),
                                  view(grad_logits, "grad_logits"), normalize, call.stream()),
           "ftrainMoeRouteBackward");
@@ -204,15 +217,15 @@ Tensor clipGradNorm(const std::vector<Tensor>& grads, double max_norm, double ep
         out_views[i] = in_views[i];
         out_views[i].memory = o.data_ptr();
     }
-    Tensor norm    = call.make({1}, at::kFloat);
+    Tensor norm    = call.make({}, at::kFloat);
     uint64_t bytes = 0;
     check(ftrainClipGradNormWorkspaceBytes(&bytes), "ftrainClipGradNormWorkspaceBytes");
-    const Tensor workspace = call.workspace(bytes);
-    check(ftrainClipGradNorm(in_views.data(), out_views.data(), static_cast<uint32_t>(grads.size()), view(norm, "norm"),
-                             static_cast<float>(max_norm), static_cast<float>(eps), workspace.data_ptr(), bytes,
+    const c10::DataPtr workspace = call.workspace(bytes);
+    check(ftrainClipGradNorm(in_views.data(), out_views.data(), static_cast<uint32_t>(grads.size()), viewOne(norm, "norm"),
+                             static_cast<float>(max_norm), static_cast<float>(eps), workspace.get(), bytes,
                              call.stream()),
           "ftrainClipGradNorm");
-    return norm.squeeze(0);
+    return norm;
 }
 
 }  // namespace
