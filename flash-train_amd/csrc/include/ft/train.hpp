@@ -18,15 +18,20 @@ namespace ftrain::train {
 
 inline std::size_t elementBytes(FTrainNumericType t) { return t == FTRAIN_NUMERIC_TYPE_FP32 ? 4 : 2; }
 
-// Launches `kernel` with the arguments it declares; a failed launch raises INTERNAL_ERROR.
+// Launches `kernel` with the arguments it declares and `lds` bytes besides its own; a failed launch raises
+// INTERNAL_ERROR.
 template <class... P>
-void launch(void (*kernel)(P...), const char* name, dim3 grid, dim3 block, hipStream_t stream, P... args) {
+void launchWithLds(void (*kernel)(P...), const char* name, dim3 grid, dim3 block, size_t lds, hipStream_t stream, P... args) {
     void* pointers[] = {static_cast<void*>(&args)...};
-    const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, pointers, 0, stream);
+    const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, pointers, lds, stream);
     if (e != hipSuccess) {
         (void)hipGetLastError();
         raise(FTRAIN_STATUS_INTERNAL_ERROR, "%s launch failed: %s", name, hipGetErrorString(e));
     }
+}
+template <class... P>
+void launch(void (*kernel)(P...), const char* name, dim3 grid, dim3 block, hipStream_t stream, P... args) {
+    launchWithLds(kernel, name, grid, block, 0, stream, args...);
 }
 
 // A device matrix whose rows are contiguous, `ld` elements apart.

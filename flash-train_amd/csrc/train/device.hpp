@@ -89,6 +89,25 @@ template <int G, class V>
 __device__ __forceinline__ V groupSum(V v) {
     return groupReduce<G>(v, [](V a, V b) { return a + b; });
 }
+// The sum over the lanes that are the same in their groups of G, in each of them (DPP: rotations of 16 lanes).
+template <int G>
+__device__ __forceinline__ float acrossGroups(float v) {
+    if constexpr (G <= 8) v += permuted<0x128>(v);
+    if constexpr (G <= 4) v += permuted<0x124>(v);
+    if constexpr (G <= 2) v += permuted<0x122>(v);
+    if constexpr (G <= 1) v += permuted<0x121>(v);
+    if constexpr (G <= 16) {
+        unsigned x = __builtin_bit_cast(unsigned, v), y = x;
+        swap16(x, y);
+        v = __builtin_bit_cast(float, x) + __builtin_bit_cast(float, y);
+    }
+    if constexpr (G <= 32) {
+        unsigned x = __builtin_bit_cast(unsigned, v), y = x;
+        swap32(x, y);
+        v = __builtin_bit_cast(float, x) + __builtin_bit_cast(float, y);
+    }
+    return v;
+}
 // One wave's LDS accesses are done in order; this keeps the compiler from moving them across.
 __device__ __forceinline__ void waveFence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

@@ -34,7 +34,7 @@ constexpr int kCus     = 256;
 // choose 46.8, scan 9.7 and place 10.0 us at 131072 x 256 instead of 44.3, 7.6 and 7.7.
 constexpr int kMaxBlocks = 4 * kCus;
 // Which form the forward pass takes (moeRouteForward): passes of one workgroup over rows, and counts.
-constexpr uint64_t kWholePasses = 4, kScanPasses = 8, kScanCounts = 32768;
+constexpr uint64_t kWholePasses = 2, kScanPasses = 8, kScanCounts = 32768;
 // Workgroups of the form without `scan`.
 constexpr int kMidBlocks = kCus;
 
@@ -232,26 +232,43 @@ struct Candidates {
     }
 };
 
+// Of a workgroup's threads, what each adds to the routed rows, the choices and sum_e counts_e sum_t p_te:
+// the launch's results from them.
+template <int THREADS>
+__device__ __forceinline__ void finishLoss(const RouteArgs& a, int routed, int choices, float dot) {
+    constexpr int kWaves = THREADS / kWave;
+    __shared__ int of_routed[kWaves], of_choices[kWaves];
+    __shared__ float of_dot[kWaves];
+    routed         = groupSum<kWave>(routed);
+    choices        = groupSum<kWave>(choices);
+    dot            = groupSum<kWave>(dot);
+    const int wave = threadIdx.x / kWave;
+    if (threadIdx.x % kWave == 0) of_routed[wave] = routed, of_choices[wave] = choices, of_dot[wave] = dot;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) routed += of_routed[w], choices += of_choices[w], dot += of_dot[w];
+        *a.routed = routed;
+        *a.loss   = static_cast<float>(a.n_experts) * (dot / static_cast<float>(max(choices, 1))) / static_cast<float>(max(routed, 1));
+    }
+}
+
 // What `choose` and `place` keep in LDS (one workgroup may do both, one after the other).
 struct ChooseLds {
-    int hist[kMaxExperts];
-    union {
-        alignas(16) unsigned rows[kThreads * 16 + kThreads];  // Candidates: at most 32 rows, 16 words apart
-        float sums[kThreads * 16];                            // after them
-    };
-    int routed[kThreads];
+    alignas(16) unsigned rows[kThreads * 16 + kThreads];  // Candidates: at most 32 rows, 16 words apart
 };
 template <int THREADS>
 struct PlaceLds {
-    int first[kMaxExperts];                   // slot of the workgroup's first choice of each expert
+    int first[kMaxExperts];                  // slot of the workgroup's first choice of each expert
     int next[THREADS / kWave][kMaxExperts];  // each wave's choices, then its next slot
 };
 
+// hist: the workgroup's choices of each expert.  choices: where one workgroup has all rows, what it chose,
+// for it to place from LDS (64 x 8: 8.5 us with counts and choices through memory, 5.1 so).
 template <class T, int VPL, int G, bool VEC>
-__device__ __forceinline__ void chooseRows(const RouteArgs& a, ChooseLds& lds) {
+__device__ __forceinline__ void chooseRows(const RouteArgs& a, ChooseLds& lds, int* hist, int16_t* choices) {
     constexpr int kRows = kThreads / G;  // rows at a time
-    int* const hist   = lds.hist;
-    float* const sums = lds.sums;
+    const bool whole    = a.blocks == 1;
     const int group = threadIdx.x / G, n = a.n_experts;
     Row<T, VPL, G, VEC> row;
     row.g = threadIdx.x % G;
@@ -287,6 +304,7 @@ __device__ __forceinline__ void chooseRows(const RouteArgs& a, ChooseLds& lds) {
             for (int k = row.g; k < a.top_k; k += G) {
                 experts[k] = -1;
                 gates[k]   = 0.f;
+                if (whole) choices[t * a.top_k + k] = -1;
             }
             continue;
         }
@@ -322,27 +340,53 @@ __device__ __forceinline__ void chooseRows(const RouteArgs& a, ChooseLds& lds) {
         for (int s = 0; s < kSlots; ++s) {
             const int k = s * G + row.g;
             if (k < a.top_k) {
-                experts[k] = at[s] < n ? at[s] : -1;
-                gates[k]   = gate[s];
-                if (at[s] < n) atomicAdd(&hist[at[s]], 1);
+                const int e = at[s] < n ? at[s] : -1;
+                experts[k]  = e;
+                gates[k]    = gate[s];
+                if (e >= 0) atomicAdd(&hist[e], 1);
+                if (whole) choices[t * a.top_k + k] = static_cast<int16_t>(e);
             }
         }
     }
-    __syncthreads();
+    // Each wave's rows, then the waves.
 #pragma unroll
-    for (int j = 0; j < VPL; ++j) sums[group * (G * VPL) + row.index(j)] = sum_p[j];
-    if (row.g == 0) lds.routed[group] = routed;
+    for (int j = 0; j < VPL; ++j) sum_p[j] = acrossGroups<G>(sum_p[j]);
+    routed = row.g == 0 ? routed : 0;
     __syncthreads();
-    for (int e = threadIdx.x; e < n; e += kThreads) {
-        float s = 0.f;
-        for (int r = 0; r < kRows; ++r) s += sums[r * (G * VPL) + e];
-        a.block_count[static_cast<int64_t>(blockIdx.x) * n + e] = hist[e];
-        a.block_p[static_cast<int64_t>(blockIdx.x) * n + e]     = s;
+    float* const sums = reinterpret_cast<float*>(lds.rows);  // [kWaves][G * VPL]
+    if (threadIdx.x % kWave < G) {
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) sums[threadIdx.x / kWave * (G * VPL) + row.index(j)] = sum_p[j];
     }
-    if (threadIdx.x == 0) {
-        int s = 0;
-        for (int r = 0; r < kRows; ++r) s += lds.routed[r];
-        a.block_routed[blockIdx.x] = s;
+    __syncthreads();
+    int chosen = 0;
+    float dot  = 0.f;
+    for (int e = threadIdx.x; e < n; e += kThreads) {
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) sum += sums[w * (G * VPL) + e];
+        const int c = hist[e];
+        if (whole) {
+            a.counts[e] = c;
+            chosen += c;
+            dot += static_cast<float>(c) * sum;
+        } else {
+            a.block_count[static_cast<int64_t>(blockIdx.x) * n + e] = c;
+            a.block_p[static_cast<int64_t>(blockIdx.x) * n + e]     = sum;
+        }
+    }
+    if (whole) {
+        finishLoss<kThreads>(a, routed, chosen, dot);
+    } else {
+        __shared__ int of_waves[kWaves];
+        routed = groupSum<kWave>(routed);
+        if (threadIdx.x % kWave == 0) of_waves[threadIdx.x / kWave] = routed;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+#pragma unroll
+            for (int w = 1; w < kWaves; ++w) routed += of_waves[w];
+            a.block_routed[blockIdx.x] = routed;
+        }
     }
 }
 
@@ -425,25 +469,36 @@ __global__ __launch_bounds__(kScanThreads) void scan(RouteArgs a) {
     }
 }
 
-// The slots of the workgroup's choices; workgroup 0 also finishes the loss.  SCANNED: `scan` has run;
-// else every workgroup adds up the others' counts by itself.
-template <bool SCANNED, int THREADS>
-__device__ __forceinline__ void placeRows(const RouteArgs& a, PlaceLds<THREADS>& lds) {
+// Where the counts are from which the slots follow: the only workgroup's own; those of each workgroup, which
+// every one adds up by itself; what `scan` has made of these.
+enum class Counts { kOwn, kEach, kScanned };
+// kEach: of how many threads an expert's counts are added up.
+template <int THREADS>
+__device__ __forceinline__ int partsOf(int experts) {
+    return experts <= THREADS / 8 ? 8 : experts <= THREADS / 2 ? 2 : 1;
+}
+
+// The slots of the workgroup's choices.  kOwn: with the choices and their counts from LDS.
+template <Counts FORM, int THREADS>
+__device__ __forceinline__ void placeRows(const RouteArgs& a, PlaceLds<THREADS>& lds, const int* own, const int16_t* choices) {
     constexpr int kThreads = THREADS, kWaves = THREADS / kWave;
     int* const first = lds.first;
     auto& next       = lds.next;
     const int n = a.n_experts, lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    if constexpr (!SCANNED) {
+    const int64_t begin = static_cast<int64_t>(blockIdx.x) * a.rows_per_block * a.top_k;
+    const int64_t end   = min(begin + static_cast<int64_t>(a.rows_per_block) * a.top_k, a.rows * a.top_k);
+    const int per_wave  = static_cast<int>((end - begin + kThreads - 1) / kThreads) * kWave;
+    const int64_t mine = min(begin + static_cast<int64_t>(wave) * per_wave, end), stop = min(mine + per_wave, end);
+    auto chosen = [&](int64_t i) -> int { return i >= stop ? -1 : FORM == Counts::kOwn ? choices[i] : a.experts[i]; };
+    const int ahead = chosen(mine + lane);  // under way with the counts
+    if constexpr (FORM == Counts::kEach) {
         // A thread an expert, or several: adjacent threads adjacent experts, each with the workgroups
         // from `part` on in steps of `parts`.
-        const int parts = n <= kThreads / 8 ? 8 : n <= kThreads / 2 ? 2 : 1;
-        const int part = threadIdx.x / (kThreads / parts), self = blockIdx.x;
+        const int parts = partsOf<kThreads>(n), part = threadIdx.x / (kThreads / parts), self = blockIdx.x;
         __shared__ int all_of[kThreads], before_of[kThreads];
-        __shared__ float sum_of[kThreads];
         for (int e0 = 0; e0 < n; e0 += kThreads / parts) {
             const int e = e0 + threadIdx.x % (kThreads / parts);
             int all = 0, before = 0;
-            float sum = 0.f;
             if (e < n) {
 #pragma unroll 16
                 for (int b = part; b < a.blocks; b += parts) {
@@ -451,72 +506,42 @@ __device__ __forceinline__ void placeRows(const RouteArgs& a, PlaceLds<THREADS>&
                     all += c;
                     before += b < self ? c : 0;
                 }
-                if (self == 0) {
-#pragma unroll 16
-                    for (int b = part; b < a.blocks; b += parts) sum += a.block_p[static_cast<int64_t>(b) * n + e];
-                }
             }
             all_of[threadIdx.x]    = all;
             before_of[threadIdx.x] = before;
-            sum_of[threadIdx.x]    = sum;
             __syncthreads();
             if (part == 0 && e < n) {
                 for (int q = 1; q < parts; ++q) {
                     all += all_of[threadIdx.x + q * (kThreads / parts)];
                     before += before_of[threadIdx.x + q * (kThreads / parts)];
-                    sum += sum_of[threadIdx.x + q * (kThreads / parts)];
                 }
                 next[0][e] = all;
                 next[1][e] = before;
-                next[2][e] = __builtin_bit_cast(int, sum);
-                if (self == 0) a.counts[e] = all;
             }
             __syncthreads();
         }
     }
-    auto count_of = [&](int e) { return SCANNED ? a.counts[e] : next[0][e]; };
-    if (blockIdx.x == 0) {
-        __shared__ float part[kWaves];
-        int routed = 0, total = 0;
-        for (int b = threadIdx.x; b < a.blocks; b += kThreads) routed += a.block_routed[b];
-        float dot = 0.f;
-        for (int e = threadIdx.x; e < n; e += kThreads) {
-            const int c = count_of(e);
-            total += c;
-            dot += static_cast<float>(c) * (SCANNED ? a.sum_p[e] : __builtin_bit_cast(float, next[2][e]));
-        }
-        int all_routed, all;
-        (void)blockScan<THREADS>(routed, all_routed);
-        (void)blockScan<THREADS>(total, all);
-        dot = groupSum<kWave>(dot);
-        if (lane == 0) part[wave] = dot;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            for (int w = 1; w < kWaves; ++w) dot += part[w];
-            *a.routed = all_routed;
-            *a.loss   = static_cast<float>(n) * (dot / static_cast<float>(max(all, 1))) / static_cast<float>(max(all_routed, 1));
-        }
-    }
+    auto count_of = [&](int e) { return FORM == Counts::kOwn ? own[e] : FORM == Counts::kEach ? next[0][e] : a.counts[e]; };
+    auto before_of = [&](int e) {
+        return FORM == Counts::kOwn    ? 0
+               : FORM == Counts::kEach ? next[1][e]
+                                       : a.block_count[static_cast<int64_t>(blockIdx.x) * n + e];
+    };
     int before = 0;
     for (int e0 = 0; e0 < n; e0 += kThreads) {
         const int e = e0 + threadIdx.x;
         int total;
-        const int at = blockScan<THREADS>(e < n ? count_of(e) : 0, total);
-        if (e < n)
-            first[e] = before + at +
-                       (SCANNED ? a.block_count[static_cast<int64_t>(blockIdx.x) * n + e] : next[1][e]);
+        const int of_blocks = e < n ? before_of(e) : 0;
+        const int at        = blockScan<THREADS>(e < n ? count_of(e) : 0, total);
+        if (e < n) first[e] = before + at + of_blocks;
         before += total;
     }
     __syncthreads();
     for (int e = threadIdx.x; e < n; e += kThreads)
         for (int w = 0; w < kWaves; ++w) next[w][e] = 0;
     __syncthreads();
-    const int64_t begin = static_cast<int64_t>(blockIdx.x) * a.rows_per_block * a.top_k;
-    const int64_t end   = min(begin + static_cast<int64_t>(a.rows_per_block) * a.top_k, a.rows * a.top_k);
-    const int per_wave  = static_cast<int>((end - begin + kThreads - 1) / kThreads) * kWave;
-    const int64_t mine = min(begin + static_cast<int64_t>(wave) * per_wave, end), stop = min(mine + per_wave, end);
-    for (int64_t i = mine + lane; i < stop; i += kWave) {
-        const int e = a.experts[i];
+    for (int64_t i0 = mine; i0 < stop; i0 += kWave) {
+        const int e = i0 == mine ? ahead : chosen(i0 + lane);
         if (e >= 0) atomicAdd(&next[wave][e], 1);
     }
     __syncthreads();
@@ -531,7 +556,7 @@ __device__ __forceinline__ void placeRows(const RouteArgs& a, PlaceLds<THREADS>&
     __syncthreads();
     for (int64_t i0 = mine; i0 < stop; i0 += kWave) {
         const int64_t i = i0 + lane;
-        const int e     = i < stop ? a.experts[i] : -1;
+        const int e     = i0 == mine ? ahead : chosen(i);
         // The lanes with the same expert: agreement in every bit of its index.
         unsigned long long peers = __ballot(e >= 0);
         for (int bit = 1; bit < n; bit <<= 1) {
@@ -549,27 +574,78 @@ __device__ __forceinline__ void placeRows(const RouteArgs& a, PlaceLds<THREADS>&
     }
 }
 
+// The routed rows and the loss, by a workgroup of its own; without `scan` also the counts.
+template <bool SCANNED, int THREADS>
+__device__ __forceinline__ void lossOfBlocks(const RouteArgs& a) {
+    const int n = a.n_experts;
+    int routed = 0, choices = 0;
+    float dot = 0.f;
+    for (int b = threadIdx.x; b < a.blocks; b += THREADS) routed += a.block_routed[b];
+    if constexpr (SCANNED) {
+        for (int e = threadIdx.x; e < n; e += THREADS) {
+            const int c = a.counts[e];
+            choices += c;
+            dot += static_cast<float>(c) * a.sum_p[e];
+        }
+    } else {
+        const int parts = partsOf<THREADS>(n), part = threadIdx.x / (THREADS / parts);
+        __shared__ int all_of[THREADS];
+        __shared__ float sum_of[THREADS];
+        for (int e0 = 0; e0 < n; e0 += THREADS / parts) {
+            const int e = e0 + threadIdx.x % (THREADS / parts);
+            int all     = 0;
+            float sum   = 0.f;
+            if (e < n) {
+#pragma unroll 16
+                for (int b = part; b < a.blocks; b += parts) {
+                    all += a.block_count[static_cast<int64_t>(b) * n + e];
+                    sum += a.block_p[static_cast<int64_t>(b) * n + e];
+                }
+            }
+            all_of[threadIdx.x] = all;
+            sum_of[threadIdx.x] = sum;
+            __syncthreads();
+            if (part == 0 && e < n) {
+                for (int q = 1; q < parts; ++q) {
+                    all += all_of[threadIdx.x + q * (THREADS / parts)];
+                    sum += sum_of[threadIdx.x + q * (THREADS / parts)];
+                }
+                a.counts[e] = all;
+                choices += all;
+                dot += static_cast<float>(all) * sum;
+            }
+            __syncthreads();
+        }
+    }
+    finishLoss<THREADS>(a, routed, choices, dot);
+}
+
 // One workgroup that has all rows goes on to place them.
 template <class T, int VPL, int G, bool VEC>
 __global__ __launch_bounds__(kThreads) void choose(RouteArgs a) {
+    __shared__ int hist[kMaxExperts];
     __shared__ union {
         ChooseLds choose;
         PlaceLds<kThreads> place;
     } lds;
-    chooseRows<T, VPL, G, VEC>(a, lds.choose);
+    extern __shared__ int16_t choices[];  // one workgroup: rows x top_k
+    chooseRows<T, VPL, G, VEC>(a, lds.choose, hist, choices);
     if (a.blocks > 1) return;
-    // The workgroup's own stores are there for it after the barrier.
     __syncthreads();
-    placeRows<false, kThreads>(a, lds.place);
+    placeRows<Counts::kOwn, kThreads>(a, lds.place, hist, choices);
 }
 
 // 131072 x 256, top 8 (16384 x 64, top 2): 8.3 us (8.1) with 256 threads, 7.4 (6.9) with 512, 10.8 (10.7)
-// with 1024.
+// with 1024; 7.1 (5.4) with 512, the choices under way with the counts and the loss to a workgroup of its own.
 constexpr int kPlaceThreads = 512;
 template <bool SCANNED>
 __global__ __launch_bounds__(kPlaceThreads) void place(RouteArgs a) {
+    if (static_cast<int>(blockIdx.x) == a.blocks) {
+        lossOfBlocks<SCANNED, kPlaceThreads>(a);
+        return;
+    }
     __shared__ PlaceLds<kPlaceThreads> lds;
-    placeRows<SCANNED, kPlaceThreads>(a, lds);
+    placeRows<SCANNED ? Counts::kScanned : Counts::kEach, kPlaceThreads>(a, lds, nullptr, nullptr);
 }
 
 template <class T, int VPL, int G, bool VEC>
@@ -745,8 +821,10 @@ void moeRouteForward(const MoeRoute& p, void* workspace, hipStream_t stream) {
     const Kernel kernel =
         kernelFor<false>(p.type, vectorRows(p.logits, p.type), static_cast<int>(p.logits.cols), lanes);
     // Whole passes of the workgroup over its rows, in one of three forms:
-    //   few passes in all: one workgroup does everything, in one launch (64 x 8: 15.8 us in three
-    //     launches, 9.0 in one);
+    //   few passes in all: one workgroup does everything, in one launch.  us of the device in one launch
+    //     of 1, 2, 3 and 4 passes, against two launches: 8 experts, top 2 5.7, 7.6, 9.5, 11.5 / 7.6; 64,
+    //     top 2 5.0, 5.9, 7.1, 8.1 / 7.4; 256, top 8 6.8, 8.9, 11.6, 13.8 / 11.6; 1024, top 8 8.7, 11.5,
+    //     14.5, 17.3 / 13.4;
     //   as many workgroups as CUs, while the counts that each of `place` then reads (one of every
     //     workgroup and expert) stay few: two launches (16384 x 64: 15.2 us in three, 13.5 in two);
     //   four workgroups on each CU, and `scan` between.
@@ -760,13 +838,13 @@ void moeRouteForward(const MoeRoute& p, void* workspace, hipStream_t stream) {
     a.block_p              = reinterpret_cast<float*>(a.block_count + p.logits.cols * kMaxBlocks);
     a.block_routed         = reinterpret_cast<int32_t*>(a.block_p + p.logits.cols * kMaxBlocks);
     a.sum_p                = reinterpret_cast<float*>(a.block_routed + kMaxBlocks);
-    launch(kernel, "router choose", dim3(a.blocks), dim3(kThreads), stream, a);
+    launchWithLds(kernel, "router choose", dim3(a.blocks), dim3(kThreads), whole ? a.rows * a.top_k * sizeof(int16_t) : 0, stream, a);
     if (a.blocks == 1) return;
     if (scanned) {
         launch(&scan, "router scan", dim3(static_cast<uint32_t>(ceilDiv(a.n_experts, kScanExperts))), dim3(kScanThreads), stream, a);
-        launch(&place<true>, "router place", dim3(a.blocks), dim3(kPlaceThreads), stream, a);
+        launch(&place<true>, "router place", dim3(a.blocks + 1), dim3(kPlaceThreads), stream, a);
     } else {
-        launch(&place<false>, "router place", dim3(a.blocks), dim3(kPlaceThreads), stream, a);
+        launch(&place<false>, "router place", dim3(a.blocks + 1), dim3(kPlaceThreads), stream, a);
     }
 }
 
