@@ -214,6 +214,13 @@ static __device__ __attribute__((aligned(256))) u16 dma_dummy[512];
 // workgroup's LDS of both operands (NB stages each), free once the workgroup has met at a barrier, and
 // the tile's first row and column.
 struct StoreTile {};
+
+// A workgroup's LDS of a and b; tiles of one size in one kernel have the same.
+template <int NB, int STAGE>
+static __shared__ __attribute__((aligned(1024))) u16 a_stages[NB][STAGE];
+template <int NB, int STAGE>
+static __shared__ __attribute__((aligned(1024))) u16 b_stages[NB][STAGE];
+
 template <bool BF16, bool TA, bool TB, int T = 128, bool SPLIT = false, int BM = T, int NB = 2, bool ROTATE = false,
           class END = StoreTile>
 // band: tile rows per band of the tile order (tile_of).
@@ -226,8 +233,6 @@ __device__ __forceinline__ void half_gemm_dma_tile(const HalfGemmParams& p, int 
     constexpr int NBM = BM / 64, NBN = T / 64;  // 32x32 blocks per wave row / column
     constexpr int NDA = BM / 32, NDB = T / 32;  // DMAs per wave per stage: A, B
     constexpr int kStageA = BM * kStageK, kStageB = T * kStageK;  // one operand, one stage
-    __shared__ __attribute__((aligned(1024))) u16 As[NB][kStageA];
-    __shared__ __attribute__((aligned(1024))) u16 Bs[NB][kStageB];
     const int tid = threadIdx.x, lane = tid & 63, li = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wrow = (wave >> 1) * (BM / 2), wcol = (wave & 1) * (T / 2);
@@ -256,8 +261,8 @@ __device__ __forceinline__ void half_gemm_dma_tile(const HalfGemmParams& p, int 
         opa.init(dma_dummy, 0, 0, BM, wave, lane);
         opb.init(dma_dummy, 0, 0, T, wave, lane);
     }
-    const unsigned la = (unsigned)(uintptr_t)(__attribute__((address_space(3))) u16*)&As[0][0];
-    const unsigned lb = (unsigned)(uintptr_t)(__attribute__((address_space(3))) u16*)&Bs[0][0];
+    const unsigned la = (unsigned)(uintptr_t)(__attribute__((address_space(3))) u16*)&a_stages<NB, kStageA>[0][0];
+    const unsigned lb = (unsigned)(uintptr_t)(__attribute__((address_space(3))) u16*)&b_stages<NB, kStageB>[0][0];
 
     // Operand of k-step ks (0..3 in the stage) for rows (or columns) x .. x + 31.
     const int tr_k = (lane & 15) >> 2, tr_x = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
@@ -363,16 +368,16 @@ __device__ __forceinline__ void half_gemm_dma_tile(const HalfGemmParams& p, int 
         for (int d = 0; d < ND; ++d) dma_one(min(i, last_st), d, i);
     static_assert((NB - 1) * ND <= 63, "the wait count field holds 63");
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NB - 1) * ND) : "memory");
-    read_half(fa0, fb0, As[0], Bs[0], 0);
+    read_half(fa0, fb0, a_stages<NB, kStageA>[0], b_stages<NB, kStageB>[0], 0);
 
     // Stage st in buffer X (a constant): the wait for the next stage leaves the NB - 2 after it in
     // flight, and the freed buffer takes the stage NB ahead.  Stages past the last reload the last
     // one (harmless: nothing reads them).
     auto phase = [&](auto x_tag, int st) {
         constexpr int X = decltype(x_tag)::value, Y = (X + 1) % NB;
-        run_half(fa0, fb0, fa1, fb1, As[X], Bs[X], 1, std::false_type{}, 0, 0);
+        run_half(fa0, fb0, fa1, fb1, a_stages<NB, kStageA>[X], b_stages<NB, kStageB>[X], 1, std::false_type{}, 0, 0);
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NB - 2) * ND) : "memory");
-        run_half(fa1, fb1, fa0, fb0, As[Y], Bs[Y], 0, std::true_type{}, min(st + NB, last_st), X);
+        run_half(fa1, fb1, fa0, fb0, a_stages<NB, kStageA>[Y], b_stages<NB, kStageB>[Y], 0, std::true_type{}, min(st + NB, last_st), X);
     };
     int st = 0;
     for (; st + NB - 1 < nst; st += NB) each<0, NB>([&](auto x) { phase(x, st + decltype(x)::value); });
@@ -391,17 +396,17 @@ __device__ __forceinline__ void half_gemm_dma_tile(const HalfGemmParams& p, int 
         opa.init(pa, p.lda, m0, MX, wave, lane);
         opb.init(pb, p.ldb, n0, NX, wave, lane);
 #pragma unroll
-        for (int j = 0; j < NDA; ++j) opa.fill(nst, j, As[0], wave, lane, k_tail);
+        for (int j = 0; j < NDA; ++j) opa.fill(nst, j, a_stages<NB, kStageA>[0], wave, lane, k_tail);
 #pragma unroll
-        for (int j = 0; j < NDB; ++j) opb.fill(nst, j, Bs[0], wave, lane, k_tail);
+        for (int j = 0; j < NDB; ++j) opb.fill(nst, j, b_stages<NB, kStageB>[0], wave, lane, k_tail);
         __syncthreads();
-        read_half(fa0, fb0, As[0], Bs[0], 0);
-        run_half(fa0, fb0, fa1, fb1, As[0], Bs[0], 1, std::false_type{}, 0, 0);
-        run_half(fa1, fb1, fa0, fb0, As[0], Bs[0], 0, std::false_type{}, 0, 0);
+        read_half(fa0, fb0, a_stages<NB, kStageA>[0], b_stages<NB, kStageB>[0], 0);
+        run_half(fa0, fb0, fa1, fb1, a_stages<NB, kStageA>[0], b_stages<NB, kStageB>[0], 1, std::false_type{}, 0, 0);
+        run_half(fa1, fb1, fa0, fb0, a_stages<NB, kStageA>[0], b_stages<NB, kStageB>[0], 0, std::false_type{}, 0, 0);
     }
 
     if constexpr (!std::is_same_v<END, StoreTile>) {
-        end(acc, reinterpret_cast<char*>(As), reinterpret_cast<char*>(Bs), m0, n0);
+        end(acc, reinterpret_cast<char*>(a_stages<NB, kStageA>), reinterpret_cast<char*>(b_stages<NB, kStageB>), m0, n0);
         return;
     }
 

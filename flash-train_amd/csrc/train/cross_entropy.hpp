@@ -68,5 +68,8 @@ struct HeadTileArgs {
 void launchHeadTileFp32(HeadTile what, int rows, const HeadTileArgs& args, int slices, hipStream_t stream);
 void launchHeadTileBf16(HeadTile what, int rows, const HeadTileArgs& args, int slices, hipStream_t stream);
 void launchHeadTileFp16(HeadTile what, int rows, const HeadTileArgs& args, int slices, hipStream_t stream);
+// kGradHidden and kGradWeight, both on tiles of 128 rows, in one launch.
+void launchHeadGradientsBf16(const HeadTileArgs& hidden, int slices, const HeadTileArgs& weight, hipStream_t stream);
+void launchHeadGradientsFp16(const HeadTileArgs& hidden, int slices, const HeadTileArgs& weight, hipStream_t stream);
 
 }  // namespace ftrain::train

@@ -7,4 +7,8 @@ void launchHeadTileBf16(HeadTile what, int rows, const HeadTileArgs& args, int s
     launchHeadTileHalf<true>(what, rows, args, slices, stream);
 }
 
+void launchHeadGradientsBf16(const HeadTileArgs& hidden, int slices, const HeadTileArgs& weight, hipStream_t stream) {
+    launchHeadGradientsHalf<true>(hidden, slices, weight, stream);
+}
+
 }  // namespace ftrain::train

@@ -7,4 +7,8 @@ void launchHeadTileFp16(HeadTile what, int rows, const HeadTileArgs& args, int s
     launchHeadTileHalf<false>(what, rows, args, slices, stream);
 }
 
+void launchHeadGradientsFp16(const HeadTileArgs& hidden, int slices, const HeadTileArgs& weight, hipStream_t stream) {
+    launchHeadGradientsHalf<false>(hidden, slices, weight, stream);
+}
+
 }  // namespace ftrain::train

@@ -433,7 +433,7 @@ struct GradWeightEnd {
 // Of the launch's parameters, those of this workgroup's tile; false: no such tile (fewer rows are
 // packed than tokens).
 template <HeadTile WHAT, class P>
-__device__ __forceinline__ bool tileProblem(const HeadTileArgs& h, P& p, int size, int tile_cols) {
+__device__ __forceinline__ bool tileProblem(const HeadTileArgs& h, P& p, int size, int tile_cols, int tile) {
     const int valid = h.head->valid * (WHAT == HeadTile::kGradHidden || WHAT == HeadTile::kGradWeight ? h.pair : 1);
     p.m = h.m, p.n = h.n, p.k = h.k;
     p.lda = h.lda, p.ldb = h.ldb, p.ldd = p.ldc = h.ldd;
@@ -445,14 +445,14 @@ __device__ __forceinline__ bool tileProblem(const HeadTileArgs& h, P& p, int siz
         p.m = min(p.m, valid);
     p.tiles_m = (p.m + size - 1) / size;
     p.tiles_n = (p.n + tile_cols - 1) / tile_cols;
-    return static_cast<int>(blockIdx.x) < p.tiles_m * p.tiles_n;
+    return tile < p.tiles_m * p.tiles_n;
 }
 
 template <bool BF16, HeadTile WHAT>
 __global__ __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_per_eu(2, 2))) void headTileHalf(HeadTileArgs h) {
     using T = std::conditional_t<BF16, bf16, fp16>;
     gemm::HalfGemmParams p{};
-    if (!tileProblem<WHAT>(h, p, 256, 256)) return;
+    if (!tileProblem<WHAT>(h, p, 256, 256, blockIdx.x)) return;
     p.a = h.a, p.b = h.b, p.d = h.d;
     using gemm::ppdev::half_gemm_pp_tile;
     using gemm::ppdev::kBand;
@@ -478,6 +478,33 @@ __global__ __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_pe
     }
 }
 
+// Tile `tile` of slice z of dx, with NB stage buffers.
+template <bool BF16, int BM, int NB>
+__device__ __forceinline__ void gradHiddenTile(const HeadTileArgs& h, int tile, int z) {
+    using T = std::conditional_t<BF16, bf16, fp16>;
+    gemm::HalfGemmParams p{};
+    if (!tileProblem<HeadTile::kGradHidden>(h, p, BM, 128, tile)) return;
+    const int first = z * h.k_chunk;
+    p.a             = static_cast<const T*>(h.a) + first;
+    p.b             = static_cast<const T*>(h.b) + first * h.ldb;
+    p.k             = max(0, min(h.k_chunk, h.k - first));
+    p.d             = static_cast<float*>(h.d) + z * h.slice;
+    if (h.add) p.c = p.d;
+    gemm::ddev::half_gemm_dma_tile<BF16, false, false, 128, false, BM, NB>(p, tile);
+}
+
+// Tile `tile` of dw.  Two stage buffers, two workgroups to a CU: k, the tokens, is short.
+template <bool BF16>
+__device__ __forceinline__ void gradWeightTile(const HeadTileArgs& h, int tile) {
+    using T   = std::conditional_t<BF16, bf16, fp16>;
+    using End = GradWeightEnd128<BF16>;
+    gemm::HalfGemmParams p{};
+    if (!tileProblem<HeadTile::kGradWeight>(h, p, 128, 128, tile)) return;
+    p.a = h.a, p.b = h.b;
+    gemm::ddev::half_gemm_dma_tile<BF16, true, false, 128, false, 128, 2, false, End>(
+        p, tile, 0, 8, End{static_cast<T*>(h.d), h.ldd, p.m, p.n, h.head->inv_scale}, h.read_m, h.read_n);
+}
+
 // BM 128: three stage buffers, as this tile runs where there are few workgroups to a CU (one needs two
 // stages in flight to be busy by itself).  BM 64, two on a CU, for at most 64 tokens, whose products are
 // the weight's reading: 16 x 4096 x 32003 bf16 loss, 262 MB, 76 -> 58 us.
@@ -486,39 +513,43 @@ __global__ __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_pe
 template <bool BF16, HeadTile WHAT, int BM>
 __global__ __launch_bounds__(256, BM == 64 || WHAT == HeadTile::kGradWeight ? 2 : 1) void headTileHalf128(HeadTileArgs h) {
     using T = std::conditional_t<BF16, bf16, fp16>;
-    gemm::HalfGemmParams p{};
-    if (!tileProblem<WHAT>(h, p, BM, 128)) return;
-    p.a = h.a, p.b = h.b, p.d = h.d;
     using gemm::ddev::half_gemm_dma_tile;
-    if constexpr (WHAT == HeadTile::kLogSum) {
-        using End = LogSumEnd128<BM>;
-        half_gemm_dma_tile<BF16, false, true, 128, false, BM, 3, true, End>(
-            p, blockIdx.x, 0, 8, End{h.rows, h.part, h.hit, h.tokens, p.m, p.n, h.first_class});
-    } else if constexpr (WHAT == HeadTile::kGradLogits) {
-        using End = GradLogitsEnd128<BF16, BM>;
-        half_gemm_dma_tile<BF16, false, true, 128, false, BM, 3, true, End>(
-            p, blockIdx.x, 0, 8, End{h.rows, static_cast<T*>(h.d), h.ldd, p.m, p.n, (h.n + 7) & ~7, h.first_class});
-    } else if constexpr (WHAT == HeadTile::kGradHidden) {
-        const int first = blockIdx.z * h.k_chunk;
-        p.a             = static_cast<const T*>(h.a) + first;
-        p.b             = static_cast<const T*>(h.b) + first * h.ldb;
-        p.k             = max(0, min(h.k_chunk, h.k - first));
-        p.d             = static_cast<float*>(h.d) + blockIdx.z * h.slice;
-        if (h.add) p.c = p.d;
-        half_gemm_dma_tile<BF16, false, false, 128, false, BM, 3>(p, blockIdx.x);
-    } else if constexpr (WHAT == HeadTile::kLogits) {
-        const int first = blockIdx.z * h.k_chunk;
-        p.a             = static_cast<const T*>(h.a) + first;
-        p.b             = static_cast<const T*>(h.b) + first;
-        p.k             = max(0, min(h.k_chunk, h.k - first));
-        p.d             = static_cast<float*>(h.d) + blockIdx.z * h.slice;
-        half_gemm_dma_tile<BF16, false, true, 128, false, BM, 3, true>(p, blockIdx.x);
+    if constexpr (WHAT == HeadTile::kGradHidden) {
+        gradHiddenTile<BF16, BM, 3>(h, blockIdx.x, blockIdx.z);
+    } else if constexpr (WHAT == HeadTile::kGradWeight) {
+        gradWeightTile<BF16>(h, blockIdx.x);
     } else {
-        // Two stage buffers, two workgroups to a CU: k, the tokens, is short.
-        using End = GradWeightEnd128<BF16>;
-        half_gemm_dma_tile<BF16, true, false, 128, false, 128, 2, false, End>(
-            p, blockIdx.x, 0, 8, End{static_cast<T*>(h.d), h.ldd, p.m, p.n, h.head->inv_scale}, h.read_m, h.read_n);
+        gemm::HalfGemmParams p{};
+        if (!tileProblem<WHAT>(h, p, BM, 128, blockIdx.x)) return;
+        p.a = h.a, p.b = h.b, p.d = h.d;
+        if constexpr (WHAT == HeadTile::kLogSum) {
+            using End = LogSumEnd128<BM>;
+            half_gemm_dma_tile<BF16, false, true, 128, false, BM, 3, true, End>(
+                p, blockIdx.x, 0, 8, End{h.rows, h.part, h.hit, h.tokens, p.m, p.n, h.first_class});
+        } else if constexpr (WHAT == HeadTile::kGradLogits) {
+            using End = GradLogitsEnd128<BF16, BM>;
+            half_gemm_dma_tile<BF16, false, true, 128, false, BM, 3, true, End>(
+                p, blockIdx.x, 0, 8, End{h.rows, static_cast<T*>(h.d), h.ldd, p.m, p.n, (h.n + 7) & ~7, h.first_class});
+        } else {
+            const int first = blockIdx.z * h.k_chunk;
+            p.a             = static_cast<const T*>(h.a) + first;
+            p.b             = static_cast<const T*>(h.b) + first;
+            p.k             = max(0, min(h.k_chunk, h.k - first));
+            p.d             = static_cast<float*>(h.d) + blockIdx.z * h.slice;
+            half_gemm_dma_tile<BF16, false, true, 128, false, BM, 3, true>(p, blockIdx.x);
+        }
     }
+}
+
+// dx's slices, `tiles` workgroups each, then dw's tiles: one launch for the two products of dl where both
+// are on this tile.
+template <bool BF16>
+__global__ __launch_bounds__(256, 2) void headGradients(HeadTileArgs hidden, HeadTileArgs weight, int tiles, int slices) {
+    const int at = static_cast<int>(blockIdx.x) - tiles * slices;
+    if (at < 0)
+        gradHiddenTile<BF16, 128, 2>(hidden, blockIdx.x % tiles, blockIdx.x / tiles);
+    else
+        gradWeightTile<BF16>(weight, at);
 }
 
 // Sums of k in one chain, as in the GEMM itself: dl's error is that of an fp32 product's logits (5e-6 of
@@ -528,7 +559,7 @@ template <HeadTile WHAT, int BM>
 __global__ __launch_bounds__(256, 2) void headTileFp32(HeadTileArgs h) {
     constexpr int WM = BM == 128 ? 2 : 4, WN = BM == 128 ? 2 : 1;
     gemm::GemmParams p{};
-    if (!tileProblem<WHAT>(h, p, BM, BM)) return;
+    if (!tileProblem<WHAT>(h, p, BM, BM, blockIdx.x)) return;
     p.a = static_cast<const float*>(h.a), p.b = static_cast<const float*>(h.b), p.d = static_cast<float*>(h.d);
     using gemm::d32::fp32_gemm_dma_tile;
     using gemm::d32::StoreTile;
@@ -564,12 +595,16 @@ __global__ __launch_bounds__(256, 2) void headTileFp32(HeadTileArgs h) {
     }
 }
 
+inline uint32_t headTiles(const HeadTileArgs& a, int rows, int cols) {
+    const int64_t tiles = (static_cast<int64_t>(a.m) + rows - 1) / rows * ((static_cast<int64_t>(a.n) + cols - 1) / cols);
+    if (tiles > INT32_MAX / 2) raise(FTRAIN_STATUS_UNSUPPORTED, "cross entropy: too many tiles (%lld)", (long long)tiles);
+    return static_cast<uint32_t>(tiles);
+}
+
 template <class K>
 void launchHead(K kernel, const char* name, const HeadTileArgs& a, int rows, int cols, int threads, int slices,
                 hipStream_t stream) {
-    const int64_t tiles = (static_cast<int64_t>(a.m) + rows - 1) / rows * ((static_cast<int64_t>(a.n) + cols - 1) / cols);
-    if (tiles > INT32_MAX) raise(FTRAIN_STATUS_UNSUPPORTED, "cross entropy: too many tiles (%lld)", (long long)tiles);
-    launch(kernel, name, dim3(static_cast<uint32_t>(tiles), 1, static_cast<uint32_t>(slices)), dim3(threads), stream, a);
+    launch(kernel, name, dim3(headTiles(a, rows, cols), 1, static_cast<uint32_t>(slices)), dim3(threads), stream, a);
 }
 
 constexpr const char* kHeadNames[5] = {"cross entropy loss", "cross entropy logits' gradient", "cross entropy hidden gradient",
@@ -591,6 +626,13 @@ void launchHeadTileHalf(HeadTile what, int rows, const HeadTileArgs& args, int s
         launchHead(large[i], kHeadNames[i], args, 256, 256, 512, slices, stream);
     else
         launchHead(rows == 128 ? medium[i] : small[i], kHeadNames[i], args, rows, 128, 256, slices, stream);
+}
+
+template <bool BF16>
+void launchHeadGradientsHalf(const HeadTileArgs& hidden, int slices, const HeadTileArgs& weight, hipStream_t stream) {
+    const uint32_t tiles = headTiles(hidden, 128, 128);
+    launch(&headGradients<BF16>, "cross entropy gradients", dim3(tiles * slices + headTiles(weight, 128, 128)), dim3(256), stream,
+           hidden, weight, static_cast<int>(tiles), slices);
 }
 
 }  // namespace ftrain::train
