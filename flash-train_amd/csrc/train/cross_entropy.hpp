@@ -24,6 +24,24 @@ struct RowInfo {
     int32_t target;  // -1: outside the classes
 };
 
+// Each row's target: of the packed rows or, without these, of every token.
+struct Targets {
+    const RowInfo* rows;
+    const void* target;
+    int64_t ignore_index, classes;
+    bool wide;  // int64, else int32
+
+    __device__ __forceinline__ int64_t given(int64_t token) const {
+        return wide ? static_cast<const int64_t*>(target)[token] : static_cast<int64_t>(static_cast<const int32_t*>(target)[token]);
+    }
+    // -1: outside the classes.
+    __device__ __forceinline__ int of(int64_t token) const {
+        const int64_t y = given(token);
+        return y >= 0 && y < classes ? static_cast<int>(y) : -1;
+    }
+    __device__ __forceinline__ int operator()(int64_t row) const { return rows != nullptr ? rows[row].target : of(row); }
+};
+
 // The products of the two passes.
 enum class HeadTile {
     kLogSum,      // tokens x classes: each row's maximum and sum of exponentials over a tile's classes
@@ -46,8 +64,8 @@ struct HeadTileArgs {
     int64_t lda, ldb, ldd;
     int32_t m, n, k;
     int32_t read_m, read_n;  // what the storage of transposed operands holds; 0: m, n
-    const Head* head;
-    const RowInfo* rows;
+    const Head* head;  // null: all of the tokens
+    Targets targets;
     int32_t pair;  // kGradHidden, kGradWeight: rows of dl (and x) of each packed token (kFewTokens)
     int32_t first_class;
     // kLogSum: a pair of maximum and sum of each part of the classes and, within it, of each of `tokens`

@@ -258,7 +258,7 @@ __device__ __forceinline__ void turned128(TileSums128<BM>& acc, char* a, char* b
 
 template <int BM>
 struct LogSumEnd128 {
-    const RowInfo* rows;
+    Targets targets;
     float2* part;
     float* hit;
     int64_t tokens;
@@ -269,7 +269,7 @@ struct LogSumEnd128 {
         int target[kTurns<BM>];
 #pragma unroll
         for (int t = 0; t < kTurns<BM>; ++t)
-            target[t] = rows[m0 + min(turnedRow(BM, t), rows_left - 1)].target - first_class - n0;
+            target[t] = targets(m0 + min(turnedRow(BM, t), rows_left - 1)) - first_class - n0;
         turned128<BM>(acc, a, b, [&](int t, int row, int col, float (&v)[8]) {
             float top = -INFINITY, sum = 0.f, x = 0.f;
 #pragma unroll
@@ -363,7 +363,7 @@ struct GradWeightEnd128 {
 
 // A row's largest logit and sum of exponentials over the 64 classes that 16 lanes hold.
 struct LogSumEnd32 {
-    const RowInfo* rows;
+    Targets targets;
     float2* part;
     float* hit;
     int64_t tokens;
@@ -383,7 +383,7 @@ struct LogSumEnd32 {
         for (int e = 0; e < 4; ++e) sum += expFast(v[e] - base);
         sum = groupSum<16>(sum);
         if (!inside) return;
-        const int at = rows[row].target - first_class - col;
+        const int at = targets(row) - first_class - col;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             if (e == at && e < left) hit[row] = v[e];
@@ -434,7 +434,8 @@ struct GradWeightEnd {
 // packed than tokens).
 template <HeadTile WHAT, class P>
 __device__ __forceinline__ bool tileProblem(const HeadTileArgs& h, P& p, int size, int tile_cols, int tile) {
-    const int valid = h.head->valid * (WHAT == HeadTile::kGradHidden || WHAT == HeadTile::kGradWeight ? h.pair : 1);
+    constexpr bool kOfDl = WHAT == HeadTile::kGradHidden || WHAT == HeadTile::kGradWeight;
+    const int valid      = h.head == nullptr ? h.m : h.head->valid * (kOfDl ? h.pair : 1);
     p.m = h.m, p.n = h.n, p.k = h.k;
     p.lda = h.lda, p.ldb = h.ldb, p.ldd = p.ldc = h.ldd;
     p.alpha = p.beta = 1.f;
@@ -458,11 +459,11 @@ __global__ __attribute__((amdgpu_flat_work_group_size(512, 512), amdgpu_waves_pe
     using gemm::ppdev::kBand;
     if constexpr (WHAT == HeadTile::kLogSum) {
         half_gemm_pp_tile<BF16, false, true>(p, blockIdx.x, kBand,
-                                             LogSumEnd16{h.rows, h.part, h.hit, h.tokens, p.m, p.n, h.first_class});
+                                             LogSumEnd16{h.targets.rows, h.part, h.hit, h.tokens, p.m, p.n, h.first_class});
     } else if constexpr (WHAT == HeadTile::kGradLogits) {
         half_gemm_pp_tile<BF16, false, true>(
             p, blockIdx.x, kBand,
-            GradLogitsEnd16<BF16>{h.rows, static_cast<T*>(h.d), h.ldd, p.m, p.n, (h.n + 7) & ~7, h.first_class});
+            GradLogitsEnd16<BF16>{h.targets.rows, static_cast<T*>(h.d), h.ldd, p.m, p.n, (h.n + 7) & ~7, h.first_class});
     } else if constexpr (WHAT == HeadTile::kGradHidden) {
         const int first = blockIdx.z * h.k_chunk;
         p.a             = static_cast<const T*>(h.a) + first;
@@ -525,11 +526,11 @@ __global__ __launch_bounds__(256, BM == 64 || WHAT == HeadTile::kGradWeight ? 2 
         if constexpr (WHAT == HeadTile::kLogSum) {
             using End = LogSumEnd128<BM>;
             half_gemm_dma_tile<BF16, false, true, 128, false, BM, 3, true, End>(
-                p, blockIdx.x, 0, 8, End{h.rows, h.part, h.hit, h.tokens, p.m, p.n, h.first_class});
+                p, blockIdx.x, 0, 8, End{h.targets, h.part, h.hit, h.tokens, p.m, p.n, h.first_class});
         } else if constexpr (WHAT == HeadTile::kGradLogits) {
             using End = GradLogitsEnd128<BF16, BM>;
             half_gemm_dma_tile<BF16, false, true, 128, false, BM, 3, true, End>(
-                p, blockIdx.x, 0, 8, End{h.rows, static_cast<T*>(h.d), h.ldd, p.m, p.n, (h.n + 7) & ~7, h.first_class});
+                p, blockIdx.x, 0, 8, End{h.targets.rows, static_cast<T*>(h.d), h.ldd, p.m, p.n, (h.n + 7) & ~7, h.first_class});
         } else {
             const int first = blockIdx.z * h.k_chunk;
             p.a             = static_cast<const T*>(h.a) + first;
@@ -566,11 +567,11 @@ __global__ __launch_bounds__(256, 2) void headTileFp32(HeadTileArgs h) {
     if constexpr (WHAT == HeadTile::kLogSum) {
         using End = LogSumEnd32;
         fp32_gemm_dma_tile<BM, BM, WM, WN, false, true, false, false, End>(
-            p, blockIdx.x, 0, 4, End{h.rows, h.part, h.hit, h.tokens, h.first_class});
+            p, blockIdx.x, 0, 4, End{h.targets, h.part, h.hit, h.tokens, h.first_class});
     } else if constexpr (WHAT == HeadTile::kGradLogits) {
         using End = GradLogitsEnd32;
         fp32_gemm_dma_tile<BM, BM, WM, WN, false, true, false, false, End>(
-            p, blockIdx.x, 0, 4, End{h.rows, static_cast<float*>(h.d), h.ldd, (h.n + 3) & ~3, h.first_class});
+            p, blockIdx.x, 0, 4, End{h.targets.rows, static_cast<float*>(h.d), h.ldd, (h.n + 3) & ~3, h.first_class});
     } else if constexpr (WHAT == HeadTile::kGradHidden) {
         const int first = blockIdx.z * h.k_chunk;
         p.a += first;
