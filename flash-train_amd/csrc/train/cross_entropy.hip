@@ -332,9 +332,17 @@ double tileMicros(bool fp32, HeadTile what, int rows, int cols, int64_t m, int64
     // 200 x 4096 x 10000 47.9 against 41.5, 16 x 4096 x 32003 113 against 80.
     if (what == HeadTile::kGradWeight && rows == 128)
         return static_cast<double>(ceilDiv(ceilDiv(m, rows) * ceilDiv(n, cols), 2 * kCus)) * (static_cast<double>(k) / 64 * 0.8 + 10.0);
-    const double stage = fp32 ? (rows == 128 ? 1.75 : 0.5) : rows == 256 ? (m <= 128 ? 0.75 : 1.25) : rows == 128 ? 0.5 : 0.3;
-    const double ends  = fp32 ? 5.0 : rows == 256 ? 9.0 : 6.0;
-    const uint64_t rounds = ceilDiv(ceilDiv(m, rows) * ceilDiv(n, cols) * slices, kCus);
+    const uint64_t tiles = ceilDiv(m, rows) * ceilDiv(n, cols) * slices;
+    // The 64x128 tile runs two to a CU; loss (gradients) with 128x128 / 64x128 of 65 x 512 x 1000 bf16 15.6 /
+    // 13.1 (26.2 / 24.2), 256 x 256 x 256 14.7 / 12.7 (20.2 / 18.0), 200 x 4096 x 10000 41.2 / 47.7 (117 / 121),
+    // 700 x 2048 x 4000 30.4 / 32.7 (76 / 78), 1000 x 1024 x 8000 36.3 / 35.5 (97.5 / 91.7).
+    const bool twice = !fp32 && rows == 64 && tiles > kCus;
+    const double stage = fp32 ? (rows == 128 ? 1.75 : 0.5)
+                         : rows == 256 ? (m <= 128 ? 0.75 : 1.25)
+                         : rows == 128 ? 0.5
+                                       : (twice ? 0.58 : 0.3);
+    const double ends = fp32 ? 5.0 : rows == 256 ? 9.0 : rows == 128 && what == HeadTile::kGradLogits ? 8.0 : 6.0;
+    const uint64_t rounds = ceilDiv(tiles, (twice ? 2 : 1) * kCus);
     return static_cast<double>(rounds) * (static_cast<double>(ceilDiv(k, slices)) / (fp32 ? 32 : 64) * stage + ends);
 }
 
@@ -373,6 +381,7 @@ Tiling tilingOf(FTrainNumericType type, HeadTile what, int64_t m, int64_t n, int
     } else {
         consider(fp32 ? 128 : 256, fp32 ? 128 : 256, fp32 ? 2 : 1);
         consider(fp32 ? 64 : 128, fp32 ? 64 : 128, fp32 ? 2 : 1);
+        if (!fp32 && !hidden && what != HeadTile::kGradWeight) consider(64, 128, 2);
     }
     return best;
 }

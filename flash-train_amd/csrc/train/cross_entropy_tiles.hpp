@@ -296,7 +296,7 @@ struct GradLogitsEnd128 {
     const RowInfo* rows;
     T* d;
     int64_t ldd;
-    int M, N, padded, first_class;
+    int M, N, padded, first_class, pair;
 
     __device__ __forceinline__ void operator()(TileSums128<BM>& acc, char* a, char* b, int m0, int n0) const {
         using gemm::ppdev::pack2;
@@ -314,15 +314,14 @@ struct GradLogitsEnd128 {
                 if (col + e >= cols_left) v[e] = 0.f;
             }
             if (row >= rows_left || n0 + col >= padded) return;
-            // Two rows a token on the 64-row tile (kFewTokens).
-            constexpr int kPair = BM == 64 ? 2 : 1;
-            T* const to         = d + (m0 + row) * kPair * ldd + n0 + col;
-            auto store          = [&](T* at) {
+            // One or two rows a token (kFewTokens).
+            T* const to = d + (m0 + row) * pair * ldd + n0 + col;
+            auto store  = [&](T* at) {
                 *reinterpret_cast<gemm::ppdev::u32x4*>(at) = gemm::ppdev::u32x4{
                     pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]), pack2<BF16>(v[4], v[5]), pack2<BF16>(v[6], v[7])};
             };
             store(to);
-            if constexpr (kPair == 2) {
+            if (pair == 2) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] -= toFloat(static_cast<T>(v[e]));
                 store(to + ldd);
@@ -508,7 +507,7 @@ __device__ __forceinline__ void gradWeightTile(const HeadTileArgs& h, int tile) 
 
 // BM 128: three stage buffers, as this tile runs where there are few workgroups to a CU (one needs two
 // stages in flight to be busy by itself).  BM 64, two on a CU, for at most 64 tokens, whose products are
-// the weight's reading: 16 x 4096 x 32003 bf16 loss, 262 MB, 76 -> 58 us.
+// the weight's reading (16 x 4096 x 32003 bf16 loss, 262 MB, 76 -> 58 us), and for the logits of few tiles.
 // ROTATE: neighbouring column tiles start at different stages, or all workgroups would read the same few
 // HBM channels at once where the weight's rows are a power of two apart.
 template <bool BF16, HeadTile WHAT, int BM>
@@ -530,7 +529,7 @@ __global__ __launch_bounds__(256, BM == 64 || WHAT == HeadTile::kGradWeight ? 2 
         } else if constexpr (WHAT == HeadTile::kGradLogits) {
             using End = GradLogitsEnd128<BF16, BM>;
             half_gemm_dma_tile<BF16, false, true, 128, false, BM, 3, true, End>(
-                p, blockIdx.x, 0, 8, End{h.targets.rows, static_cast<T*>(h.d), h.ldd, p.m, p.n, (h.n + 7) & ~7, h.first_class});
+                p, blockIdx.x, 0, 8, End{h.targets.rows, static_cast<T*>(h.d), h.ldd, p.m, p.n, (h.n + 7) & ~7, h.first_class, h.pair});
         } else {
             const int first = blockIdx.z * h.k_chunk;
             p.a             = static_cast<const T*>(h.a) + first;
