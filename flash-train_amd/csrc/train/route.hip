@@ -27,14 +27,16 @@
 namespace ftrain::train {
 namespace {
 
-constexpr int kThreads = 256;
+// Threads of a workgroup that chooses, of one of the backward pass.  Of 256 twice the workgroups choose, and
+// their counts are twice as many: 131072 x 256, top 8 61.4 us, 59.9 with 512; 16384 x 64, top 2 10.5 and 10.2.
+constexpr int kThreads = 512, kBackThreads = 256;
 constexpr int kWaves   = kThreads / kWave;
 constexpr int kCus     = 256;
-// Most workgroups: as many as are on the chip at once with the registers of the widest rows.  Six a CU:
-// choose 46.8, scan 9.7 and place 10.0 us at 131072 x 256 instead of 44.3, 7.6 and 7.7.
-constexpr int kMaxBlocks = 4 * kCus;
+// Most workgroups: as many as are on the chip at once with the registers of the widest rows.  Half as many
+// again: choose 46.8, scan 9.7 and place 10.0 us at 131072 x 256 instead of 44.3, 7.6 and 7.7.
+constexpr int kMaxBlocks = 2 * kCus;
 // Which form the forward pass takes (moeRouteForward): passes of one workgroup over rows, and counts.
-constexpr uint64_t kWholePasses = 2, kScanPasses = 8, kScanCounts = 32768;
+constexpr uint64_t kWholePasses = 2, kScanPasses = 4, kScanCounts = 32768;
 // Workgroups of the form without `scan`.
 constexpr int kMidBlocks = kCus;
 
@@ -255,7 +257,7 @@ __device__ __forceinline__ void finishLoss(const RouteArgs& a, int routed, int c
 
 // What `choose` and `place` keep in LDS (one workgroup may do both, one after the other).
 struct ChooseLds {
-    alignas(16) unsigned rows[kThreads * 16 + kThreads];  // Candidates: at most 32 rows, 16 words apart
+    alignas(16) unsigned rows[kThreads * 16 + kThreads];  // Candidates: at most 64 rows, 16 words apart
 };
 template <int THREADS>
 struct PlaceLds {
@@ -391,7 +393,7 @@ __device__ __forceinline__ void chooseRows(const RouteArgs& a, ChooseLds& lds, i
 }
 
 // Exclusive prefix sum of one value a thread over the workgroup; total: the sum.
-template <int THREADS = kThreads>
+template <int THREADS>
 __device__ __forceinline__ int blockScan(int v, int& total) {
     constexpr int kWaves = THREADS / kWave;
     __shared__ int wave_sum[kWaves];
@@ -649,18 +651,18 @@ __global__ __launch_bounds__(kPlaceThreads) void place(RouteArgs a) {
 }
 
 template <class T, int VPL, int G, bool VEC>
-__global__ __launch_bounds__(kThreads) void backward(RouteArgs a) {
-    constexpr int kRows = kThreads / G;
+__global__ __launch_bounds__(kBackThreads) void backward(RouteArgs a) {
+    constexpr int kRows = kBackThreads / G;
     // Of each group's row: p, and what its choices add to the gradient.
-    __shared__ __attribute__((aligned(16))) float row_p[kThreads * VPL], row_add[kThreads * VPL];
+    __shared__ __attribute__((aligned(16))) float row_p[kBackThreads * VPL], row_add[kBackThreads * VPL];
     const int group = threadIdx.x / G, n = a.n_experts;
     Row<T, VPL, G, VEC> row;
     row.g              = threadIdx.x % G;
     float* const all_p = row_p + group * (G * VPL);
     float* const add   = row_add + group * (G * VPL);
     int total = 0, all;
-    for (int e = threadIdx.x; e < n; e += kThreads) total += a.counts[e];
-    (void)blockScan(total, all);
+    for (int e = threadIdx.x; e < n; e += kBackThreads) total += a.counts[e];
+    (void)blockScan<kBackThreads>(total, all);
     // d loss / d p_te
     const float factor = *a.grad_loss * static_cast<float>(n) / static_cast<float>(max(all, 1)) /
                          static_cast<float>(max(*a.routed, 1));
@@ -822,12 +824,12 @@ void moeRouteForward(const MoeRoute& p, void* workspace, hipStream_t stream) {
         kernelFor<false>(p.type, vectorRows(p.logits, p.type), static_cast<int>(p.logits.cols), lanes);
     // Whole passes of the workgroup over its rows, in one of three forms:
     //   few passes in all: one workgroup does everything, in one launch.  us of the device in one launch
-    //     of 1, 2, 3 and 4 passes, against two launches: 8 experts, top 2 5.7, 7.6, 9.5, 11.5 / 7.6; 64,
-    //     top 2 5.0, 5.9, 7.1, 8.1 / 7.4; 256, top 8 6.8, 8.9, 11.6, 13.8 / 11.6; 1024, top 8 8.7, 11.5,
-    //     14.5, 17.3 / 13.4;
+    //     of one pass and of two, against two launches: 8 experts, top 2 6.4, 8.7 / 8.4; 64, top 2 5.6,
+    //     6.8 / 7.4; 64 fp32, top 8 6.8, 9.4 / 8.9; 256, top 8 7.8, 10.5 / 12.3; 1024, top 8 8.9, 12.2 /
+    //     13.7 (and the host's 2.4 for a launch);
     //   as many workgroups as CUs, while the counts that each of `place` then reads (one of every
     //     workgroup and expert) stay few: two launches (16384 x 64: 15.2 us in three, 13.5 in two);
-    //   four workgroups on each CU, and `scan` between.
+    //   two workgroups on each CU, and `scan` between.
     const uint64_t at_once = kThreads / lanes, all = ceilDiv(a.rows, at_once);
     const bool whole       = all <= kWholePasses;
     const bool scanned     = !whole && (all > kScanPasses * kMidBlocks || p.logits.cols * kMidBlocks > kScanCounts);
@@ -854,9 +856,9 @@ void moeRouteBackward(const MoeRoute& p, hipStream_t stream) {
     int lanes = 0;
     const bool vec = vectorRows(p.logits, p.type) && vectorRows(p.grad_logits, p.type);
     const Kernel kernel    = kernelFor<true>(p.type, vec, static_cast<int>(p.logits.cols), lanes);
-    const uint64_t at_once = kThreads / lanes;
-    launch(kernel, "router backward", dim3(static_cast<uint32_t>(std::min<uint64_t>(ceilDiv(a.rows, at_once), 2 * kMaxBlocks))),
-           dim3(kThreads), stream, a);
+    const uint64_t at_once = kBackThreads / lanes;
+    launch(kernel, "router backward", dim3(static_cast<uint32_t>(std::min<uint64_t>(ceilDiv(a.rows, at_once), 8 * kCus))),
+           dim3(kBackThreads), stream, a);
 }
 
 }  // namespace ftrain::train
