@@ -9,8 +9,8 @@
 //
 // A token whose target is the ignored index takes no part: the others' rows of x are packed densely
 // first, so neither its hidden state (whatever is in it) nor its work reaches any sum.  Where x lies
-// and how it is aligned is thereby settled too.  A target outside the classes makes its token's loss
-// and gradients NaN.
+// and how it is aligned is thereby settled too.  (The loss of few tokens goes without: Layout::direct.)
+// A target outside the classes makes its token's loss and gradients NaN.
 #include <algorithm>
 
 #include "cross_entropy.hpp"

@@ -1,5 +1,5 @@
 // The cross entropy's products on the GEMM's tiles, with the ends below in place of d = alpha acc + beta c:
-// 16-bit types on 256x256 (gemm/pingpong_tile.hpp) and 128x128 (gemm/dma_tile.hpp), fp32 on 128x128 and
+// 16-bit types on 256x256 (gemm/pingpong_tile.hpp), 128x128 and 64x128 (gemm/dma_tile.hpp), fp32 on 128x128 and
 // 64x64 (gemm/dma32_tile.hpp).
 #pragma once
 

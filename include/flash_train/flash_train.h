@@ -60,8 +60,9 @@ FTRAIN_API FTrainStatus ftrainGemmNoAlloc(FTrainStorageView a, FTrainStorageView
  * launches on `stream` only (nothing is allocated, copied or synchronised, so
  * it may be captured into a graph), and gives the same bits for the same
  * inputs.  `workspace` is device memory of at least the bytes that the
- * operator's ...WorkspaceBytes call names, aligned to 256 bytes, with any
- * contents; calls that may overlap need one each.  Errors: INVALID_ARGUMENT
+ * operator's ...WorkspaceBytes call names for the same views (their strides
+ * and alignment matter), aligned to 256 bytes, with any contents; calls that
+ * may overlap need one each.  Errors: INVALID_ARGUMENT
  * (null, shapes, host memory, workspace), UNSUPPORTED (types, strides,
  * limits), INTERNAL_ERROR (a launch failed).
  */
