@@ -217,9 +217,39 @@ def test_cross_entropy_on_every_tile(ft, shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1, 8, 3), (7, 1032, 260), (40, 64, 530), (64, 2048, 300), (64, 512, 5003)])
+def test_cross_entropy_of_few_tokens_as_they_lie(ft, shape, dtype):
+    """At most 64 tokens are not packed: rows apart, ignored tokens of any content among them, a target
+    outside the classes."""
+    x, w, y, grad = head(*shape, dtype, ignored=0.3 if shape[0] > 1 else 0.0, seed=31)
+    noisy = x.clone()
+    for i, row in enumerate(torch.nonzero(y == IGNORE)[:, 0].tolist()):
+        noisy[row] = (math.nan, math.inf, -math.inf)[i % 3]
+    for wide in (True, False):
+        target = (y if wide else y.int()).cuda()
+        check_head(ft, x, w, y, grad, device=(strided(noisy, 8, 0), w.cuda(), target, grad.cuda()))
+    y[-1] = shape[2]
+    loss, lse = ft.linear_cross_entropy_forward(noisy.cuda(), w.cuda(), y.cuda())
+    bad = torch.arange(shape[0]) == shape[0] - 1
+    assert torch.equal(torch.isnan(loss).cpu(), bad) and (loss.cpu()[y == IGNORE] == 0).all()
+    # An ignored index that is a class.
+    y[:] = 2
+    loss, lse = ft.linear_cross_entropy_forward(noisy.cuda(), w.cuda(), y.cuda(), ignore_index=2)
+    assert (loss == 0).all() and (lse == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(65, 520, 1003), (200, 264, 513), (256, 256, 256), (500, 1024, 5003), (600, 72, 300),
+                                   (2000, 512, 1500)])
+def test_cross_entropy_gradients_in_one_launch(ft, shape, dtype):
+    """Sizes where both products of dl share a launch, with slices of the classes and without."""
+    check_head(ft, *head(*shape, dtype, ignored=0.1, seed=37))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("hidden", [64, 59])
 def test_cross_entropy_in_several_pieces(ft, hidden, dtype):
-    """dl of 8192 tokens in pieces of 16384 (16-bit) or 8192 classes; 59: the weight's rows are packed too."""
+    """dl of 8192 tokens in pieces of 32768 (16-bit) or 16384 classes; 59: the weight's rows are packed too."""
     x, w, y, grad = head(8192, hidden, 40003, dtype, ignored=0.1, seed=23)
     dev = [t.cuda() for t in (x, w, y, grad)]
     loss, lse = ft.linear_cross_entropy_forward(*dev[:3])
@@ -292,6 +322,18 @@ def check_route(ft, logits, top_k, normalize, mask=None, device=None):
 def test_route(ft, rows, n, top_k, dtype):
     for normalize in (False, True):
         check_route(ft, router_logits(rows, n, dtype, seed=rows + n), top_k, normalize)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,top_k,passes", [(8, 2, 512), (8, 8, 512), (20, 5, 128), (64, 2, 64), (128, 32, 32), (256, 8, 32),
+                                            (260, 4, 16), (1024, 32, 8)])
+def test_route_in_one_launch_and_in_two(ft, n, top_k, passes, dtype):
+    """Around the most rows that one workgroup takes, twice `passes`."""
+    for rows in (passes, passes + 1, 2 * passes - 1, 2 * passes, 2 * passes + 1):
+        logits = router_logits(rows, n, dtype, seed=rows)
+        mask = torch.rand(rows, generator=torch.Generator().manual_seed(rows)) < 0.8
+        logits[rows // 2] = -math.inf
+        check_route(ft, logits, top_k, True, mask)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
