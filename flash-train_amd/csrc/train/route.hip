@@ -88,10 +88,10 @@ struct Row {
     }
     __device__ __forceinline__ void unpack(int n) {
 #pragma unroll
-        for (int j = 0; j < VPL; ++j) {
-            const T x = VEC ? static_cast<T>(raw[VEC ? j / kVec : 0][j % kVec]) : one[VEC ? 0 : j];
-            v[j]      = index(VEC ? j / kVec * kVec : j) < n ? toFloat(x) : -INFINITY;
-        }
+        for (int j = 0; j < VPL; ++j) v[j] = toFloat(VEC ? static_cast<T>(raw[VEC ? j / kVec : 0][j % kVec]) : one[VEC ? 0 : j]);
+        if (n == G * VPL) return;
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) v[j] = index(VEC ? j / kVec * kVec : j) < n ? v[j] : -INFINITY;
     }
     __device__ __forceinline__ void load(const T* row, int n) {
         fetch(row, n);
@@ -137,11 +137,11 @@ struct Candidates {
     static constexpr unsigned kIndex = kMaxExperts - 1, kFree = 0x1FFFu;
     static constexpr unsigned kLeast = 0x00800000u;  // the number of the lowest finite value is not less
     // Words of a row in LDS: the rows of a wave start in different banks.  A lane's run lies in 16-byte
-    // chunks, chunk c at place (c + lane / 4) mod 4 of every four, so that lanes write to different banks.
+    // chunks, chunk c at place c ^ (lane / 4 mod 4) of every four, so that lanes write to different banks.
     static constexpr int kStride = G * VPL + 16;
     static __device__ __forceinline__ int placeOf(int run, int j) {
         constexpr int kMask = VPL / 4 - 1 < 3 ? VPL / 4 - 1 : 3;
-        return run * VPL + 4 * ((j / 4 & ~kMask) | ((j / 4 + run / 4) & kMask)) + j % 4;
+        return run * VPL + (j ^ (run & 4 * kMask));
     }
     unsigned key[VPL];
     unsigned own;          // the lane's largest
