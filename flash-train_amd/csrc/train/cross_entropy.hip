@@ -134,14 +134,27 @@ __global__ __launch_bounds__(kThreads) void packWeight(const T* w, int64_t ld, i
         copyRow(w + v * ld, out + v * padded, cols, padded);
 }
 
-// Four adjacent sums, of which `left` lie in the matrix (none: nothing is read), over the slices.
-__device__ __forceinline__ void joinSlices(const float* from, int64_t slice, int slices, int left, float (&v)[4]) {
+// Four adjacent sums over the slices first, first + step .. below `end`; at(z): where slice z's are.  Four
+// loads are under way at once, the first again for those past the end (one after the other, the six slices
+// of 500 x 1024 took 5.6 us, so 4.9).
+template <class AT>
+__device__ __forceinline__ float4 sumSlices(int first, int step, int end, AT&& at) {
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (left > 0)
-        for (int z = 0; z < slices; ++z) {
-            const float4 x = *reinterpret_cast<const float4*>(from + z * slice);
-            s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
-        }
+    if (first < end && first + step >= end) return *reinterpret_cast<const float4*>(at(first));
+    for (int z0 = first; z0 < end; z0 += 4 * step) {
+        float4 x[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) x[b] = *reinterpret_cast<const float4*>(at(z0 + b * step < end ? z0 + b * step : z0));
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+            if (z0 + b * step < end) s.x += x[b].x, s.y += x[b].y, s.z += x[b].z, s.w += x[b].w;
+    }
+    return s;
+}
+
+// Four adjacent logits, of which `left` lie in the matrix (none: nothing is read).
+__device__ __forceinline__ void joinSlices(const float* from, int64_t slice, int slices, int left, float (&v)[4]) {
+    const float4 s = left > 0 ? sumSlices(0, 1, slices, [&](int z) { return from + z * slice; }) : make_float4(0.f, 0.f, 0.f, 0.f);
     v[0] = s.x, v[1] = s.y, v[2] = s.z, v[3] = s.w;
 }
 
@@ -277,12 +290,8 @@ __global__ __launch_bounds__(kThreads) void finishHidden(const float* sums, int6
         float4 v      = make_float4(0.f, 0.f, 0.f, 0.f);
         if (row >= 0 && i < cols) {
             const float* const from = sums + static_cast<int64_t>(row) * pair * ld + i;
-#pragma unroll 8
-            for (int z = MANY ? wave : 0; z < slices * pair; z += MANY ? kWaves : 1) {
-                const int64_t at = pair == 2 ? (z >> 1) * slice + (z & 1) * ld : z * slice;
-                const float4 x   = *reinterpret_cast<const float4*>(from + at);
-                v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
-            }
+            v = sumSlices(MANY ? wave : 0, MANY ? kWaves : 1, slices * pair,
+                          [&](int z) { return from + (pair == 2 ? (z >> 1) * slice + (z & 1) * ld : z * slice); });
         }
         if constexpr (MANY) {
             __syncthreads();
