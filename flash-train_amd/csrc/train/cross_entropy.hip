@@ -267,9 +267,10 @@ __global__ __launch_bounds__(kFinishThreads) void finishLoss(const float2* part,
     join(v);
     joinLanes();
     if (share != 0 || t >= tokens) return;
-    const float l = top + logf(sum);
-    lse[t]        = row < 0 ? 0.f : l;
-    loss[t]       = row < 0 ? 0.f : y < 0 ? NAN : l - l_y;
+    // Not lse - l_y: where the target holds nearly all, the loss is far smaller than the rounding of lse.
+    const float log_sum = logf(sum);
+    lse[t]              = row < 0 ? 0.f : top + log_sum;
+    loss[t]             = row < 0 ? 0.f : y < 0 ? NAN : (top - l_y) + log_sum;
 }
 
 // grad_hidden row t: the packed row's sums, rounded once; zeros for an ignored token.  A lane takes four

@@ -127,6 +127,22 @@ def test_cross_entropy_of_extreme_logits(ft, dtype):
     check_head(ft, x, w, y, grad)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens", [1, 100])
+def test_cross_entropy_small_losses_are_not_lost_in_lse(ft, tokens, dtype):
+    """Logits that are whole numbers, the target's far above: the loss is the logarithm of a sum near 1,
+    with an error of a few roundings of 1, not of the logits."""
+    x = torch.zeros(tokens, 16, dtype=dtype)
+    x[:, 0] = torch.arange(tokens) % 5 + 1.0
+    w = torch.zeros(600, 16, dtype=dtype)
+    w[7, 0], w[300, 0], w[599, 0] = 24.0, 20.0, 18.0
+    y = torch.full((tokens,), 7)
+    loss, lse = ft.linear_cross_entropy_forward(x.cuda(), w.cuda(), y.cuda())
+    exact = torch.logsumexp(x.double() @ w.double().t(), 1) - 24.0 * x[:, 0].double()
+    within(loss, exact, 16 * U32 * (1.0 + exact), "loss")
+    within(lse, exact + 24.0 * x[:, 0].double(), 16 * U32 * (1.0 + exact) + U32 * 2 * 24.0 * x[:, 0].double(), "lse")
+
+
 def test_cross_entropy_keeps_small_probabilities_in_fp16(ft):
     x, w, y, grad = head(48, 64, 6000, torch.float16, seed=12, spread=0.5)
     check_head(ft, x, w, y, grad * 2.0**-12 * 6000)  # every dl far below fp16's smallest normal number
