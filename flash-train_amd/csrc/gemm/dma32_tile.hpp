@@ -133,10 +133,12 @@ static __device__ __attribute__((aligned(256))) float dma32_dummy[512];
 // lies in the matrix; left: how many columns from `column` on do.
 // read_m, read_n: rows and columns that a's and b's storage holds, where that is more than m and n (a
 // transposed operand is read in whole chunks of 4); 0: m, n.
+// FOLD: the sums of every FOLD stages of 32 k are kept apart and then added to the total, so the error of
+// a long k grows with the roots of both counts instead of that of k.
 struct StoreTile {};
 
 template <int BM, int BN, int WM, int WN, bool SPLIT, bool TB = false, bool TA = false, bool U = false,
-          class END = StoreTile>
+          class END = StoreTile, int FOLD = 0>
 __device__ __forceinline__ void fp32_gemm_dma_tile(const GemmParams& p, int bid, int z, int band = 4, const END& end = END{},
                                                    int read_m = 0, int read_n = 0) {
     static_assert(WM * WN == 4, "4 waves");
@@ -299,6 +301,26 @@ __device__ __forceinline__ void fp32_gemm_dma_tile(const GemmParams& p, int bid,
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
 
+    static_assert(FOLD % 2 == 0, "the stage loop takes two at a time");
+    floatx4 total[FOLD > 0 ? TM : 1][FOLD > 0 ? TN : 1];
+    if constexpr (FOLD > 0) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) total[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+    auto fold = [&] {
+        if constexpr (FOLD > 0) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) {
+                    total[i][j] += acc[i][j];
+                    acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+                }
+        }
+    };
+
     // Operands of one half stage: fa[bi] (4 k-steps), fb[s][cc] (4 columns); column-major b:
     // fb[bj & 3][bj >> 2] holds block bj's 4 k-steps.
     floatx4 fa0[TM], fb0[4][NC], fa1[TM], fb1[4][NC];
@@ -386,6 +408,8 @@ __device__ __forceinline__ void fp32_gemm_dma_tile(const GemmParams& p, int bid,
         for (; st + 1 < nst; st += 2) {
             FT_DMA32_PHASE(As0, Bs0, As1, Bs1, la0, lb0, st)
             FT_DMA32_PHASE(As1, Bs1, As0, Bs0, la1, lb1, st + 1)
+            if constexpr (FOLD > 0)
+                if (st % FOLD == FOLD - 2) fold();
         }
         if (st < nst) {
             FT_DMA32_PHASE(As0, Bs0, As1, Bs1, la0, lb0, st)
@@ -453,6 +477,12 @@ __device__ __forceinline__ void fp32_gemm_dma_tile(const GemmParams& p, int bid,
         }
     }
 
+    if constexpr (FOLD > 0) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] += total[i][j];
+    }
     if constexpr (!std::is_same_v<END, StoreTile>) {
         const int rows_left = M - m0;
 #pragma unroll

@@ -552,9 +552,11 @@ __global__ __launch_bounds__(256, 2) void headGradients(HeadTileArgs hidden, Hea
         gradWeightTile<BF16>(weight, at);
 }
 
-// Sums of k in one chain, as in the GEMM itself: dl's error is that of an fp32 product's logits (5e-6 of
-// its size at k = 2048, 1.5e-5 at 8192).  Sums of 512 k added up apart took a third to a tenth of that
-// error and 5% more time (16 accumulators' worth of spills at 256 registers).
+// The logits' sums of k: on the 64x64 tile those of every 256 apart and then added up, as a loss near 0 is as
+// exact as its logits.  Root mean square errors of losses near 10, in one chain / so: 16 x 8192 x 20000 7.2e-6 /
+// 6.1e-7, 16 x 1000 x 1000 1.7e-6 / 6.3e-7, 100 x 8192 x 1000 4.7e-6 / 5.7e-7.  On the 128x128 tile in one chain, as in
+// the GEMM itself (5e-6 of dl's size at k = 2048, 1.5e-5 at 8192): there it took 5% more time (16 accumulators'
+// worth of spills at 256 registers).
 template <HeadTile WHAT, int BM>
 __global__ __launch_bounds__(256, 2) void headTileFp32(HeadTileArgs h) {
     constexpr int WM = BM == 128 ? 2 : 4, WN = BM == 128 ? 2 : 1;
@@ -563,13 +565,14 @@ __global__ __launch_bounds__(256, 2) void headTileFp32(HeadTileArgs h) {
     p.a = static_cast<const float*>(h.a), p.b = static_cast<const float*>(h.b), p.d = static_cast<float*>(h.d);
     using gemm::d32::fp32_gemm_dma_tile;
     using gemm::d32::StoreTile;
+    constexpr int kFold = BM == 64 ? 8 : 0;  // stages
     if constexpr (WHAT == HeadTile::kLogSum) {
         using End = LogSumEnd32;
-        fp32_gemm_dma_tile<BM, BM, WM, WN, false, true, false, false, End>(
+        fp32_gemm_dma_tile<BM, BM, WM, WN, false, true, false, false, End, kFold>(
             p, blockIdx.x, 0, 4, End{h.targets, h.part, h.hit, h.tokens, h.first_class});
     } else if constexpr (WHAT == HeadTile::kGradLogits) {
         using End = GradLogitsEnd32;
-        fp32_gemm_dma_tile<BM, BM, WM, WN, false, true, false, false, End>(
+        fp32_gemm_dma_tile<BM, BM, WM, WN, false, true, false, false, End, kFold>(
             p, blockIdx.x, 0, 4, End{h.targets.rows, static_cast<float*>(h.d), h.ldd, (h.n + 3) & ~3, h.first_class});
     } else if constexpr (WHAT == HeadTile::kGradHidden) {
         const int first = blockIdx.z * h.k_chunk;
@@ -587,7 +590,7 @@ __global__ __launch_bounds__(256, 2) void headTileFp32(HeadTileArgs h) {
         p.d += blockIdx.z * h.slice;
         // Whole chunks of four columns are stored; the row stride has room for them.
         p.n = (h.n + 3) & ~3;
-        fp32_gemm_dma_tile<BM, BM, WM, WN, false, true, false, false, StoreTile>(p, blockIdx.x, 0, 4, StoreTile{}, 0, h.n);
+        fp32_gemm_dma_tile<BM, BM, WM, WN, false, true, false, false, StoreTile, kFold>(p, blockIdx.x, 0, 4, StoreTile{}, 0, h.n);
     } else {
         using End = GradWeightEnd;
         fp32_gemm_dma_tile<BM, BM, WM, WN, false, false, true, false, End>(
