@@ -134,13 +134,13 @@ static __device__ __attribute__((aligned(256))) float dma32_dummy[512];
 // read_m, read_n: rows and columns that a's and b's storage holds, where that is more than m and n (a
 // transposed operand is read in whole chunks of 4); 0: m, n.
 // FOLD: the sums of every FOLD stages of 32 k are kept apart and then added to the total, so the error of
-// a long k grows with the roots of both counts instead of that of k.
+// a long k grows with the roots of both counts instead of that of k.  apart: whether they are.
 struct StoreTile {};
 
 template <int BM, int BN, int WM, int WN, bool SPLIT, bool TB = false, bool TA = false, bool U = false,
           class END = StoreTile, int FOLD = 0>
 __device__ __forceinline__ void fp32_gemm_dma_tile(const GemmParams& p, int bid, int z, int band = 4, const END& end = END{},
-                                                   int read_m = 0, int read_n = 0) {
+                                                   int read_m = 0, int read_n = 0, bool apart = true) {
     static_assert(WM * WN == 4, "4 waves");
     constexpr int WTM = BM / WM, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16, NC = TN / 4;
     static_assert(TN % 4 == 0 && TM >= 1, "column runs of four blocks");
@@ -409,7 +409,7 @@ __device__ __forceinline__ void fp32_gemm_dma_tile(const GemmParams& p, int bid,
             FT_DMA32_PHASE(As0, Bs0, As1, Bs1, la0, lb0, st)
             FT_DMA32_PHASE(As1, Bs1, As0, Bs0, la1, lb1, st + 1)
             if constexpr (FOLD > 0)
-                if (st % FOLD == FOLD - 2) fold();
+                if (apart && st % FOLD == FOLD - 2) fold();
         }
         if (st < nst) {
             FT_DMA32_PHASE(As0, Bs0, As1, Bs1, la0, lb0, st)

@@ -363,8 +363,8 @@ constexpr double kJoinMicros   = 5.0;
 // k may be cut, in slices of at least 512, until the tiles fill the device (two workgroups of fp32 and of
 // the 64x128 tile run on a CU): dx's always, as its sums are fp32 in the workspace anyway; the logits'
 // where few tokens' few tiles have a long k, at the price of writing and reading the slices (at 4 TB/s)
-// and a launch: gradients of 16 x 8192 x 4000 fp32 255 -> 146 us; also where a last round is nearly empty,
-// loss of 16 x 8192 x 20000 fp32 274 -> 198.  (With 200 x 4096 x 10000 8% of
+// and a launch: gradients of 16 x 8192 x 4000 fp32 255 -> 146 us; also where a last round is nearly
+// empty, loss of 16 x 8192 x 20000 fp32 274 -> 198.  (With 200 x 4096 x 10000 8% of
 // 528 us: not done.)
 Tiling tilingOf(FTrainNumericType type, HeadTile what, int64_t m, int64_t n, int64_t k) {
     const bool fp32 = type == FTRAIN_NUMERIC_TYPE_FP32, hidden = what == HeadTile::kGradHidden;

@@ -58,6 +58,9 @@ enum class HeadTile {
 // as the rounding of the result alone; of many tokens 1.4 times.
 constexpr int64_t kFewTokens = 64;
 
+// Up to this many tokens (fp32) dl's logits are summed apart (headTileFp32).
+constexpr int64_t kApartTokens = 128;
+
 struct HeadTileArgs {
     const void *a, *b;
     void* d;

@@ -554,9 +554,11 @@ __global__ __launch_bounds__(256, 2) void headGradients(HeadTileArgs hidden, Hea
 
 // The logits' sums of k: on the 64x64 tile those of every 256 apart and then added up, as a loss near 0 is as
 // exact as its logits.  Root mean square errors of losses near 10, in one chain / so: 16 x 8192 x 20000 7.2e-6 /
-// 6.1e-7, 16 x 1000 x 1000 1.7e-6 / 6.3e-7, 100 x 8192 x 1000 4.7e-6 / 5.7e-7.  On the 128x128 tile in one chain, as in
-// the GEMM itself (5e-6 of dl's size at k = 2048, 1.5e-5 at 8192): there it took 5% more time (16 accumulators'
-// worth of spills at 256 registers).
+// 6.1e-7, 16 x 1000 x 1000 1.7e-6 / 6.3e-7, 100 x 8192 x 1000 4.7e-6 / 5.7e-7; of dl's products, of their size,
+// 16 x 8192 x 20000 1.2e-5 / 1.5e-6, 100 x 4096 x 1000 1.5e-5 / 1.3e-6.  dl of more tokens than kApartTokens, whose
+// errors are many, and the 128x128 tile: one chain, as in the GEMM itself (5e-6 of dl's size at k = 2048, 1.5e-5
+// at 8192), which the results then agree with; on the large tile it took 5% more time (16 accumulators' worth of
+// spills at 256 registers).
 template <HeadTile WHAT, int BM>
 __global__ __launch_bounds__(256, 2) void headTileFp32(HeadTileArgs h) {
     constexpr int WM = BM == 128 ? 2 : 4, WN = BM == 128 ? 2 : 1;
@@ -573,7 +575,7 @@ __global__ __launch_bounds__(256, 2) void headTileFp32(HeadTileArgs h) {
     } else if constexpr (WHAT == HeadTile::kGradLogits) {
         using End = GradLogitsEnd32;
         fp32_gemm_dma_tile<BM, BM, WM, WN, false, true, false, false, End, kFold>(
-            p, blockIdx.x, 0, 4, End{h.targets.rows, static_cast<float*>(h.d), h.ldd, (h.n + 3) & ~3, h.first_class});
+            p, blockIdx.x, 0, 4, End{h.targets.rows, static_cast<float*>(h.d), h.ldd, (h.n + 3) & ~3, h.first_class}, 0, 0, h.m <= kApartTokens);
     } else if constexpr (WHAT == HeadTile::kGradHidden) {
         const int first = blockIdx.z * h.k_chunk;
         p.a += first;
